@@ -12,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -21,8 +22,13 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 CAPI_SO = os.path.join(LIBDIR, "libmellin_b200.so")
 TORCH_SO = os.path.join(LIBDIR, "mellin_torch.so")
 
-CAPI_SOURCES = ["capi.cu", "kernels.cu", "tc_direct.cu", "tc_direct_taps.cu", "tc_direct_masked.cu", "tc_gradw.cu", "batch_inner.cu", "gradw_rows.cu", "direct_rows.cu", "tc_scatter.cu", "tc_few_in.cu", "tc_gradw_few_in.cu", "few_in_rows.cu", "prologue.cu", "static_scratch.cu", "table_cache.cu", "peaks.cu", "index_map.cpp"]
+CAPI_SOURCES = ["capi.cu", "kernels.cu", "tc_direct.cu", "tc_direct_taps.cu", "tc_direct_masked.cu", "tc_gradw.cu", "batch_inner.cu", "gradw_rows.cu", "direct_rows.cu", "tc_scatter.cu", "tc_few_in.cu", "tc_gradw_few_in.cu", "few_in_rows.cu", "prologue.cu", "recurrence.cu", "group_norm.cu", "philox_dropout.cu", "static_scratch.cu", "table_cache.cu", "peaks.cu", "index_map.cpp"]
 CAPI_HEADERS = ["mellin_internal.h", "index_map.h", "tc_ptx.cuh", "tuning_hooks.h"]
+# headers that only some sources include
+EXTRA_DEPS = {"tc_direct_taps.cu": ["tc_direct.cu"], "tc_direct_masked.cu": ["tc_direct.cu"],
+              "recurrence.cu": ["sequence_common.cuh"], "group_norm.cu": ["sequence_common.cuh"],
+              "philox_dropout.cu": ["sequence_common.cuh"]}
+TORCH_SOURCES = ["mellin_torch.cpp", "sequence_torch.cpp"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
@@ -59,11 +65,10 @@ def _compile_object(args):
 
 def build_capi(force=False, verbose_ptxas=False):
     """Compile every source to its own object (in parallel) and link them."""
-    from concurrent.futures import ThreadPoolExecutor
-
     srcs = [os.path.join(CSRC, s) for s in CAPI_SOURCES]
     headers = [os.path.join(CSRC, h) for h in CAPI_HEADERS] + [os.path.join(INCLUDE, "mellin_b200.h")]
-    if not force and _fresh(CAPI_SO, srcs + headers):
+    extra = [os.path.join(CSRC, d) for d in sorted({d for deps in EXTRA_DEPS.values() for d in deps})]
+    if not force and _fresh(CAPI_SO, srcs + headers + extra):
         return CAPI_SO
     os.makedirs(LIBDIR, exist_ok=True)
     os.makedirs(OBJDIR, exist_ok=True)
@@ -72,8 +77,7 @@ def build_capi(force=False, verbose_ptxas=False):
     for src in srcs:
         obj = os.path.join(OBJDIR, os.path.splitext(os.path.basename(src))[0] + ".o")
         objs.append(obj)
-        # tc_direct_taps.cu / tc_direct_masked.cu include tc_direct.cu
-        deps = [src] + headers + ([os.path.join(CSRC, "tc_direct.cu")] if "tc_direct_" in src else [])
+        deps = [src] + headers + [os.path.join(CSRC, d) for d in EXTRA_DEPS.get(os.path.basename(src), [])]
         if force or not _fresh(obj, deps):
             jobs.append((src, obj, flags))
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
@@ -86,23 +90,26 @@ def build_torch_binding(force=False):
     import torch
     from torch.utils import cpp_extension
 
-    src = os.path.join(CSRC, "mellin_torch.cpp")
-    if not os.path.isfile(src):
-        return None
-    deps = [src, os.path.join(INCLUDE, "mellin_b200.h"), CAPI_SO]
-    if not force and _fresh(TORCH_SO, deps):
+    srcs = [os.path.join(CSRC, s) for s in TORCH_SOURCES]
+    header = os.path.join(INCLUDE, "mellin_b200.h")
+    if not force and _fresh(TORCH_SO, srcs + [header, CAPI_SO]):
         return TORCH_SO
     cxx = shutil.which("g++") or shutil.which("c++")
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cuda_home = cpp_extension.CUDA_HOME or "/usr/local/cuda"
     includes = cpp_extension.include_paths() + [os.path.join(cuda_home, "include"), INCLUDE]
-    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=mellin_torch",
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
+    flags = ["-O2", "-std=c++17", "-fPIC", "-DTORCH_EXTENSION_NAME=mellin_torch",
+             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
     for inc in includes:
-        cmd += ["-isystem", inc]
-    cmd += [src, "-o", TORCH_SO, "-L" + LIBDIR, "-lmellin_b200", "-Wl,-rpath,$ORIGIN",
-            "-L" + torch_lib, "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_cuda", "-lc10_cuda",
-            "-L" + os.path.join(cuda_home, "lib64"), "-lcudart"]
+        flags += ["-isystem", inc]
+    os.makedirs(OBJDIR, exist_ok=True)
+    objs = [os.path.join(OBJDIR, os.path.splitext(s)[0] + ".o") for s in TORCH_SOURCES]
+    stale = [(src, obj) for src, obj in zip(srcs, objs) if force or not _fresh(obj, [src, header])]
+    with ThreadPoolExecutor(max_workers=2) as pool:
+        list(pool.map(lambda so: _run([cxx] + flags + ["-c", so[0], "-o", so[1]]), stale))
+    cmd = [cxx, "-shared"] + objs + ["-o", TORCH_SO, "-L" + LIBDIR, "-lmellin_b200", "-Wl,-rpath,$ORIGIN",
+           "-L" + torch_lib, "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_cuda", "-lc10_cuda",
+           "-L" + os.path.join(cuda_home, "lib64"), "-lcudart"]
     _run(cmd)
     return TORCH_SO
 

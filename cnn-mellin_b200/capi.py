@@ -35,8 +35,11 @@ MISC = ["mellin_abi_version", "mellin_last_error", "mellin_launch_count", "melli
         "mellin_selftest_unarmed_wait", "mellin_selftest_fma_rate",
         "mellin_mcorrlcorr_forward_f16", "mellin_mcorrlcorr_grad_input_f16", "mellin_mcorrlcorr_grad_weight_f16",
         "mellin_mcorrlcorr_forward_workspace_bytes_f16", "mellin_mcorrlcorr_grad_input_workspace_bytes_f16",
-        "mellin_mcorrlcorr_grad_weight_workspace_bytes_f16", "mellin_lift_compress_workspace_bytes"]
+        "mellin_mcorrlcorr_grad_weight_workspace_bytes_f16", "mellin_lift_compress_workspace_bytes",
+        "mellin_gated_recurrence_state_count"]
 PROLOGUE = ["mellin_lift_compress", "mellin_lift_compress_backward"]
+SEQUENCE = ["mellin_gated_recurrence", "mellin_gated_recurrence_backward", "mellin_group_norm_act",
+            "mellin_group_norm_act_backward", "mellin_group_norm_act_workspace_bytes", "mellin_philox_dropout"]
 
 
 def exported_symbols():
@@ -44,6 +47,8 @@ def exported_symbols():
     names = list(SIZE_FUNCTIONS) + MISC
     for base in OP1D + OP2D + COL1D + COL2D + LAYER + PROLOGUE:
         names += [base + "_f32", base + "_f64"]
+    for base in SEQUENCE:
+        names += [base + sfx for sfx in ("_f32", "_f64", "_f16", "_bf16")]
     return names
 
 
@@ -74,6 +79,10 @@ def lib():
                 fn = getattr(_lib, "mellin_mcorrlcorr_%s_workspace_bytes%s" % (name, sfx))
                 fn.restype, fn.argtypes = ctypes.c_size_t, [_I64] * 17
         _lib.mellin_lift_compress_workspace_bytes.restype = ctypes.c_size_t
+        _lib.mellin_gated_recurrence_state_count.restype = _I64
+        for sfx in ("_f32", "_f64", "_f16", "_bf16"):
+            fn = getattr(_lib, "mellin_group_norm_act_workspace_bytes" + sfx)
+            fn.restype, fn.argtypes = ctypes.c_size_t, [_I64] * 3
     return _lib
 
 

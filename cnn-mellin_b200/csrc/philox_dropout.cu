@@ -1,0 +1,144 @@
+// Dropout whose mask is a function of (seed, element offset) and is never stored, with an optional residual added in the
+// same pass:
+//
+//   y[i] = (word(i) >= p * 2^32 ? x[i] / (1 - p) : 0) + residual[i]
+//
+// word(i) is word i % 4 of Philox4x32-10 (J. K. Salmon, M. A. Moraes, R. O. Dror, D. E. Shaw: Parallel random numbers:
+// as easy as 1, 2, 3; SC 2011) with counter i / 4 and the 64-bit seed as key, i the element's offset in row-major order.
+// Backward is the same pass over the gradient with the same seed and no residual.
+#include <algorithm>
+#include <cmath>
+
+#include "sequence_common.cuh"
+
+namespace mellin {
+namespace {
+
+using namespace seq;
+
+constexpr int kThreads = 256;
+
+struct Words {
+  unsigned w[4];
+};
+
+__device__ __forceinline__ Words philox4x32_10(unsigned long long counter, unsigned long long key) {
+  unsigned c0 = (unsigned)counter, c1 = (unsigned)(counter >> 32), c2 = 0, c3 = 0;
+  unsigned k0 = (unsigned)key, k1 = (unsigned)(key >> 32);
+#pragma unroll
+  for (int round = 0; round < 10; ++round) {
+    const unsigned long long p0 = (unsigned long long)0xD2511F53u * c0, p1 = (unsigned long long)0xCD9E8D57u * c2;
+    c0 = (unsigned)(p1 >> 32) ^ c1 ^ k0, c1 = (unsigned)p1;
+    c2 = (unsigned)(p0 >> 32) ^ c3 ^ k1, c3 = (unsigned)p0;
+    k0 += 0x9E3779B9u, k1 += 0xBB67AE85u;
+  }
+  return {{c0, c1, c2, c3}};
+}
+
+template <typename T>
+struct DropoutArgs {
+  const T *x = nullptr, *residual = nullptr;
+  T *y = nullptr;
+  long long rows = 0, cols = 0, x_stride = 0, r_stride = 0;  // y is dense; strides between rows, in elements
+  unsigned long long threshold = 0;                          // dropped where word < threshold; 2^32: all are
+  Acc<T> scale = 1;
+  unsigned long long seed = 0;
+  const long long *seed_device = nullptr;  // read instead of `seed` when there is one
+};
+
+// V elements a thread and turn, V a multiple of 4.  ROWS: x or the residual has rows that are not adjacent.  VEC: packed
+// accesses (everything 16-byte aligned, rows a multiple of V long); otherwise element by element.
+template <typename T, int V, bool VEC>
+__global__ void __launch_bounds__(kThreads) philox_dropout_kernel(const DropoutArgs<T> a) {
+  using A = Acc<T>;
+  const unsigned long long key = a.seed_device != nullptr ? (unsigned long long)*a.seed_device : a.seed;
+  const long long total = a.rows * a.cols, groups = (total + V - 1) / V, step = (long long)gridDim.x * kThreads;
+  for (long long g = blockIdx.x * (long long)kThreads + threadIdx.x; g < groups; g += step) {
+    const long long i = g * V;
+    Pack<T, V> x, r, o;
+    if constexpr (VEC) {
+      const long long row = a.rows == 1 ? 0 : i / a.cols, col = i - row * a.cols;
+      x = *reinterpret_cast<const Pack<T, V> *>(a.x + row * a.x_stride + col);
+      if (a.residual != nullptr) r = *reinterpret_cast<const Pack<T, V> *>(a.residual + row * a.r_stride + col);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (i + v < total) {
+          const long long row = a.rows == 1 ? 0 : (i + v) / a.cols, col = i + v - row * a.cols;
+          x.v[v] = a.x[row * a.x_stride + col];
+          if (a.residual != nullptr) r.v[v] = a.residual[row * a.r_stride + col];
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+      const Words w = philox4x32_10((unsigned long long)(i / 4 + q), key);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int v = q * 4 + j;
+        A value = w.w[j] >= a.threshold ? to_acc(x.v[v]) * a.scale : A(0);
+        if (a.residual != nullptr) value += to_acc(r.v[v]);
+        o.v[v] = from_acc<T>(value);
+      }
+    }
+    if constexpr (VEC) {
+      *reinterpret_cast<Pack<T, V> *>(a.y + i) = o;
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (i + v < total) a.y[i + v] = o.v[v];
+    }
+  }
+}
+
+template <typename T>
+int run(DropoutArgs<T> a, double p, void *stream) {
+  const char *who = "philox_dropout";
+  return guarded(who, [&]() -> int {
+    if (a.rows < 0 || a.cols < 0) return fail(MELLIN_ERR_BAD_ARGUMENT, std::string(who) + ": negative extent");
+    if (!(p >= 0.0 && p <= 1.0)) return fail(MELLIN_ERR_BAD_ARGUMENT, std::string(who) + ": p outside [0, 1]");
+    if ((long double)a.rows * (long double)a.cols > 4.0e18L)
+      return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": more than 2^62 elements");
+    const long long total = a.rows * a.cols;
+    if (total == 0) return MELLIN_OK;
+    if (a.x == nullptr || a.y == nullptr) return fail(MELLIN_ERR_BAD_ARGUMENT, std::string(who) + ": null pointer");
+    a.threshold = (unsigned long long)std::floor(p * 4294967296.0 + 0.5);
+    a.scale = p < 1.0 ? (Acc<T>)(1.0 / (1.0 - p)) : Acc<T>(0);
+    if (a.x_stride == a.cols && (a.residual == nullptr || a.r_stride == a.cols)) a.cols = total, a.rows = 1;
+    constexpr int V = sizeof(T) == 2 ? 8 : 4;
+    constexpr size_t bytes = sizeof(T) * V;
+    const bool vec = a.cols % V == 0 && aligned_to(a.x, bytes) && aligned_to(a.y, bytes) && aligned_to(a.residual, bytes) &&
+                     (a.rows == 1 || (a.x_stride % V == 0 && (a.residual == nullptr || a.r_stride % V == 0)));
+    const long long blocks = (total + (long long)V * kThreads - 1) / ((long long)V * kThreads);
+    const unsigned grid = (unsigned)std::min<long long>(blocks, 0x7fffffffLL);
+    auto st = static_cast<cudaStream_t>(stream);
+    if (vec) philox_dropout_kernel<T, V, true><<<grid, kThreads, 0, st>>>(a);
+    else philox_dropout_kernel<T, V, false><<<grid, kThreads, 0, st>>>(a);
+    return launched(who);
+  });
+}
+
+}  // namespace
+}  // namespace mellin
+
+using namespace mellin;
+
+#define DROPOUT_ENTRY(SUFFIX, T, P)                                                                                  \
+  int mellin_philox_dropout_##SUFFIX(const P *x, int64_t x_stride, const P *residual, int64_t residual_stride,       \
+                                     int64_t rows, int64_t cols, double p, uint64_t seed, const int64_t *seed_device, \
+                                     P *y, void *stream) {                                                           \
+    DropoutArgs<T> a;                                                                                                \
+    a.x = static_cast<const T *>(x), a.residual = static_cast<const T *>(residual), a.y = static_cast<T *>(y);       \
+    a.rows = rows, a.cols = cols, a.x_stride = x_stride, a.r_stride = residual_stride, a.seed = seed;                \
+    a.seed_device = reinterpret_cast<const long long *>(seed_device);                                                \
+    return run<T>(a, p, stream);                                                                                     \
+  }
+
+extern "C" {
+
+DROPOUT_ENTRY(f32, float, float)
+DROPOUT_ENTRY(f64, double, double)
+DROPOUT_ENTRY(f16, __half, void)
+DROPOUT_ENTRY(bf16, __nv_bfloat16, void)
+
+}  // extern "C"

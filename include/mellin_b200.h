@@ -295,6 +295,133 @@ int mellin_lift_compress_backward_f64(const double *x, const double *grad_y, con
                                       double *grad_tau, double *grad_eps, void *workspace, size_t workspace_bytes,
                                       void *stream);
 
+/* ---- sequence operators on per-frame features ---------------------------------
+ * What a model runs between its convolutions and its output: (batch, frames, channels) tensors whose channels are
+ * adjacent; `*_sn` / `*_st` are the strides, in elements, between utterances and between frames (a time-major tensor
+ * and half of a wider projection need no copy).  `lens` (device int32, one per utterance, or NULL: all frames exist;
+ * held inside [0, frames]) ends the utterances: frames behind the end are never read, their outputs and input
+ * gradients are written as zeros.  Suffixes f32 / f64 / f16 / bf16 name the tensors' type (`const void *` = device
+ * pointers to IEEE half / bfloat16 values); sums, states, statistics and parameters are float (double for f64).  No
+ * call allocates, blocks or synchronises: all of them can be captured into a graph.  No reference counterpart: the
+ * reference's AcousticModel uses torch's recurrent layers and dropout there (models.py:435-445). */
+
+/* Gated linear recurrence: f = sigmoid(gate), h_t = f_t h_{t-1} + (1 - f_t) x_t, y_t = h_t, over an utterance's frames,
+ * first to last or (reverse != 0) last to first.  initial: (batch, channels) state before the first frame met, or
+ * NULL: zeros.  final: receives the state after the last one, or NULL.  states: receives what backward recomputes
+ * from, mellin_gated_recurrence_state_count(...) elements, or NULL when no backward call follows.
+ * Backward: grad_y and grad_final may be NULL (zeros); grad_initial may be NULL.  grad_x and grad_gate may be the two
+ * halves of one tensor; no output may overlap an input. */
+int64_t mellin_gated_recurrence_state_count(int64_t batch, int64_t frames, int64_t channels);
+int mellin_gated_recurrence_f32(const float *x, int64_t x_sn, int64_t x_st, const float *gate, int64_t gate_sn,
+                                int64_t gate_st, const float *initial, const int *lens, int reverse, int64_t batch,
+                                int64_t frames, int64_t channels, float *y, int64_t y_sn, int64_t y_st, float *final,
+                                float *states, void *stream);
+int mellin_gated_recurrence_backward_f32(const float *x, int64_t x_sn, int64_t x_st, const float *gate, int64_t gate_sn,
+                                         int64_t gate_st, const float *states, const int *lens, int reverse,
+                                         int64_t batch, int64_t frames, int64_t channels, const float *grad_y,
+                                         int64_t grad_y_sn, int64_t grad_y_st, const float *grad_final, float *grad_x,
+                                         int64_t grad_x_sn, int64_t grad_x_st, float *grad_gate, int64_t grad_gate_sn,
+                                         int64_t grad_gate_st, float *grad_initial, void *stream);
+int mellin_gated_recurrence_f64(const double *x, int64_t x_sn, int64_t x_st, const double *gate, int64_t gate_sn,
+                                int64_t gate_st, const double *initial, const int *lens, int reverse, int64_t batch,
+                                int64_t frames, int64_t channels, double *y, int64_t y_sn, int64_t y_st, double *final,
+                                double *states, void *stream);
+int mellin_gated_recurrence_backward_f64(const double *x, int64_t x_sn, int64_t x_st, const double *gate, int64_t gate_sn,
+                                         int64_t gate_st, const double *states, const int *lens, int reverse,
+                                         int64_t batch, int64_t frames, int64_t channels, const double *grad_y,
+                                         int64_t grad_y_sn, int64_t grad_y_st, const double *grad_final, double *grad_x,
+                                         int64_t grad_x_sn, int64_t grad_x_st, double *grad_gate, int64_t grad_gate_sn,
+                                         int64_t grad_gate_st, double *grad_initial, void *stream);
+int mellin_gated_recurrence_f16(const void *x, int64_t x_sn, int64_t x_st, const void *gate, int64_t gate_sn,
+                                int64_t gate_st, const float *initial, const int *lens, int reverse, int64_t batch,
+                                int64_t frames, int64_t channels, void *y, int64_t y_sn, int64_t y_st, float *final,
+                                float *states, void *stream);
+int mellin_gated_recurrence_backward_f16(const void *x, int64_t x_sn, int64_t x_st, const void *gate, int64_t gate_sn,
+                                         int64_t gate_st, const float *states, const int *lens, int reverse,
+                                         int64_t batch, int64_t frames, int64_t channels, const void *grad_y,
+                                         int64_t grad_y_sn, int64_t grad_y_st, const float *grad_final, void *grad_x,
+                                         int64_t grad_x_sn, int64_t grad_x_st, void *grad_gate, int64_t grad_gate_sn,
+                                         int64_t grad_gate_st, float *grad_initial, void *stream);
+int mellin_gated_recurrence_bf16(const void *x, int64_t x_sn, int64_t x_st, const void *gate, int64_t gate_sn,
+                                int64_t gate_st, const float *initial, const int *lens, int reverse, int64_t batch,
+                                int64_t frames, int64_t channels, void *y, int64_t y_sn, int64_t y_st, float *final,
+                                float *states, void *stream);
+int mellin_gated_recurrence_backward_bf16(const void *x, int64_t x_sn, int64_t x_st, const void *gate, int64_t gate_sn,
+                                         int64_t gate_st, const float *states, const int *lens, int reverse,
+                                         int64_t batch, int64_t frames, int64_t channels, const void *grad_y,
+                                         int64_t grad_y_sn, int64_t grad_y_st, const float *grad_final, void *grad_x,
+                                         int64_t grad_x_sn, int64_t grad_x_st, void *grad_gate, int64_t grad_gate_sn,
+                                         int64_t grad_gate_st, float *grad_initial, void *stream);
+
+/* Group norm and an activation: y = act((x - mean) * rstd * weight[c] + bias[c]); mean and biased variance over an
+ * utterance's frames and the channels / groups adjacent channels of a group, rstd = 1 / sqrt(var + eps).  weight / bias:
+ * (channels), or NULL: ones / zeros.  act: 0 none, 1 ReLU, 2 SiLU (z sigmoid(z)), 3 GELU (z Phi(z)).  stats: receives
+ * (batch, groups, 2) mean and rstd for backward, or NULL.  workspace: mellin_group_norm_act_workspace_bytes_*() bytes,
+ * 16-byte aligned, for either call; its contents are clobbered.  Backward: grad_weight / grad_bias (channels) may be
+ * NULL; they are summed in a fixed order. */
+size_t mellin_group_norm_act_workspace_bytes_f32(int64_t batch, int64_t frames, int64_t channels);
+int mellin_group_norm_act_f32(const float *x, int64_t x_sn, int64_t x_st, const float *weight, const float *bias,
+                              const int *lens, int64_t batch, int64_t frames, int64_t channels, int64_t groups,
+                              double eps, int act, float *y, int64_t y_sn, int64_t y_st, float *stats, void *workspace,
+                              size_t workspace_bytes, void *stream);
+int mellin_group_norm_act_backward_f32(const float *x, int64_t x_sn, int64_t x_st, const float *weight, const float *bias,
+                                       const float *stats, const int *lens, int64_t batch, int64_t frames,
+                                       int64_t channels, int64_t groups, int act, const float *grad_y,
+                                       int64_t grad_y_sn, int64_t grad_y_st, float *grad_x, int64_t grad_x_sn,
+                                       int64_t grad_x_st, float *grad_weight, float *grad_bias, void *workspace,
+                                       size_t workspace_bytes, void *stream);
+size_t mellin_group_norm_act_workspace_bytes_f64(int64_t batch, int64_t frames, int64_t channels);
+int mellin_group_norm_act_f64(const double *x, int64_t x_sn, int64_t x_st, const double *weight, const double *bias,
+                              const int *lens, int64_t batch, int64_t frames, int64_t channels, int64_t groups,
+                              double eps, int act, double *y, int64_t y_sn, int64_t y_st, double *stats, void *workspace,
+                              size_t workspace_bytes, void *stream);
+int mellin_group_norm_act_backward_f64(const double *x, int64_t x_sn, int64_t x_st, const double *weight, const double *bias,
+                                       const double *stats, const int *lens, int64_t batch, int64_t frames,
+                                       int64_t channels, int64_t groups, int act, const double *grad_y,
+                                       int64_t grad_y_sn, int64_t grad_y_st, double *grad_x, int64_t grad_x_sn,
+                                       int64_t grad_x_st, double *grad_weight, double *grad_bias, void *workspace,
+                                       size_t workspace_bytes, void *stream);
+size_t mellin_group_norm_act_workspace_bytes_f16(int64_t batch, int64_t frames, int64_t channels);
+int mellin_group_norm_act_f16(const void *x, int64_t x_sn, int64_t x_st, const float *weight, const float *bias,
+                              const int *lens, int64_t batch, int64_t frames, int64_t channels, int64_t groups,
+                              double eps, int act, void *y, int64_t y_sn, int64_t y_st, float *stats, void *workspace,
+                              size_t workspace_bytes, void *stream);
+int mellin_group_norm_act_backward_f16(const void *x, int64_t x_sn, int64_t x_st, const float *weight, const float *bias,
+                                       const float *stats, const int *lens, int64_t batch, int64_t frames,
+                                       int64_t channels, int64_t groups, int act, const void *grad_y,
+                                       int64_t grad_y_sn, int64_t grad_y_st, void *grad_x, int64_t grad_x_sn,
+                                       int64_t grad_x_st, float *grad_weight, float *grad_bias, void *workspace,
+                                       size_t workspace_bytes, void *stream);
+size_t mellin_group_norm_act_workspace_bytes_bf16(int64_t batch, int64_t frames, int64_t channels);
+int mellin_group_norm_act_bf16(const void *x, int64_t x_sn, int64_t x_st, const float *weight, const float *bias,
+                              const int *lens, int64_t batch, int64_t frames, int64_t channels, int64_t groups,
+                              double eps, int act, void *y, int64_t y_sn, int64_t y_st, float *stats, void *workspace,
+                              size_t workspace_bytes, void *stream);
+int mellin_group_norm_act_backward_bf16(const void *x, int64_t x_sn, int64_t x_st, const float *weight, const float *bias,
+                                       const float *stats, const int *lens, int64_t batch, int64_t frames,
+                                       int64_t channels, int64_t groups, int act, const void *grad_y,
+                                       int64_t grad_y_sn, int64_t grad_y_st, void *grad_x, int64_t grad_x_sn,
+                                       int64_t grad_x_st, float *grad_weight, float *grad_bias, void *workspace,
+                                       size_t workspace_bytes, void *stream);
+
+/* Dropout with a mask that is a function of (seed, element offset): element i (row-major offset) is dropped where word
+ * i % 4 of Philox4x32-10 with counter i / 4 and key `seed` is below p * 2^32, and scaled by 1 / (1 - p) otherwise;
+ * residual (or NULL) is added.  A dropped element is zero whatever x holds.  x and residual are (rows, cols) with
+ * *_stride elements between rows; y is dense.  seed_device (or NULL) is a device word read instead of `seed`, so that
+ * a captured graph can draw a new mask at each replay.  Backward: the same call on the gradient, without residual. */
+int mellin_philox_dropout_f32(const float *x, int64_t x_stride, const float *residual, int64_t residual_stride,
+                              int64_t rows, int64_t cols, double p, uint64_t seed, const int64_t *seed_device, float *y,
+                              void *stream);
+int mellin_philox_dropout_f64(const double *x, int64_t x_stride, const double *residual, int64_t residual_stride,
+                              int64_t rows, int64_t cols, double p, uint64_t seed, const int64_t *seed_device, double *y,
+                              void *stream);
+int mellin_philox_dropout_f16(const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
+                              int64_t rows, int64_t cols, double p, uint64_t seed, const int64_t *seed_device, void *y,
+                              void *stream);
+int mellin_philox_dropout_bf16(const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
+                              int64_t rows, int64_t cols, double p, uint64_t seed, const int64_t *seed_device, void *y,
+                              void *stream);
+
 /* ---- diagnostics ------------------------------------------------------------ */
 
 /* Number of kernels this library has launched from the calling process since

@@ -1,0 +1,511 @@
+"""The sequence operators (``sequence.py``) on the GPU, against the float64 restatement in ``oracle/sequence_oracle.py``.
+
+Tolerances: the restatement's own error bound for float32 (float64) arithmetic, plus half a step of the output's type
+relative to the value.  Frames behind an utterance's end hold NaN, infinities and the type's lowest value in every test
+with lengths: they must not be seen.
+"""
+import numpy as np
+import pytest
+import torch
+
+import capi
+import sequence
+from oracle import sequence_oracle as so
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16, torch.float64]
+HALF_STEP = {t: torch.finfo(t).eps / 2 for t in TYPES}
+TINY = {t: torch.finfo(t).smallest_normal * torch.finfo(t).eps for t in TYPES}  # half a step below the normal range
+
+
+def _unit(dtype):
+    return 2.0 ** -53 if dtype == torch.float64 else 2.0 ** -24
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _close(got, pair, dtype, name):
+    value, bound = pair
+    got = _np(got)
+    assert got.shape == value.shape, (name, got.shape, value.shape)
+    if not value.size:
+        return
+    allowed = bound + HALF_STEP[dtype] * (np.abs(value) + bound) + TINY[dtype]
+    excess = np.abs(got - value) - allowed
+    assert np.isfinite(got).all(), name
+    worst = np.unravel_index(np.argmax(excess), excess.shape)
+    assert excess[worst] <= 0, (name, worst, got[worst], value[worst], allowed[worst])
+
+
+def _poison(t, lens):
+    """What must never be seen, behind the end of each utterance."""
+    bad = [float("nan"), float("inf"), float("-inf"), torch.finfo(t.dtype).min]
+    for i, length in enumerate(lens):
+        for j in range(max(int(length), 0), t.shape[1]):
+            t[i, j] = bad[j % 4]
+    return t
+
+
+def _laid_out(t, layout):
+    """The same values: as they are, time-major, channels of a wider tensor, or off the 16-byte grid."""
+    n, f, c = t.shape
+    if layout == "time-major":
+        return t.transpose(0, 1).contiguous().transpose(0, 1)
+    if layout == "wide":
+        wide = torch.full((n, f, 2 * c + 8), float("nan"), dtype=t.dtype, device=t.device)
+        wide[..., 8:8 + c] = t
+        return wide[..., 8:8 + c]
+    if layout == "odd":
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+        flat[1:] = t.reshape(-1)
+        return flat[1:].view(n, f, c)
+    if layout == "channels apart":
+        return t.transpose(1, 2).contiguous().transpose(1, 2)
+    return t
+
+
+# ---- gated recurrence ------------------------------------------------------------------------------------------------
+
+# (batch, frames, channels, lens, reverse, with an initial state, layout)
+RECURRENCES = [
+    (1, 1, 1, None, False, False, "dense"),
+    (3, 1, 70, None, False, True, "packed"),
+    (2, 2, 8, [2, 1], True, True, "dense"),
+    (4, 15, 33, [15, 0, 7, 1], False, True, "packed"),
+    (4, 16, 64, [16, 0, 15, 1], True, False, "packed"),
+    (3, 17, 32, [17, 16, 0], False, False, "time-major"),
+    (2, 33, 128, None, True, True, "wide"),
+    (2, 63, 40, [63, 64 + 5], False, True, "odd"),
+    (2, 64, 96, [-3, 40], True, True, "time-major"),
+    (3, 65, 24, [65, 64, 63], False, False, "channels apart"),
+    (2, 130, 256, [129, 128], True, True, "packed"),
+    (5, 257, 31, [257, 256, 255, 0, 129], False, True, "packed"),
+    (1, 1031, 16, None, True, False, "packed"),
+    (2, 700, 72, [513, 700], False, True, "dense"),
+    (1, 5000, 8, None, False, True, "packed"),
+    (70, 9, 48, [i % 10 for i in range(70)], True, False, "packed"),
+]
+
+
+def _recurrence_problem(case, dtype, seed):
+    n, t, c, lens, reverse, with_initial, layout = case
+    rng = np.random.default_rng(seed)
+
+    def tensor(*shape, mean=0.0, to=dtype):
+        return torch.from_numpy(rng.standard_normal(shape) + mean).to("cuda").to(to)
+
+    state = torch.float64 if dtype == torch.float64 else torch.float32
+    p = {"x": tensor(n, t, c), "gate": tensor(n, t, c, mean=1.0).clamp(-8, 8), "grad_y": tensor(n, t, c),
+         "grad_final": tensor(n, c, to=state), "initial": tensor(n, c, to=state) if with_initial else None}
+    want = so.recurrence(*(_np(p[k]) if p[k] is not None else None for k in ("x", "gate", "initial")), lens, reverse,
+                         _np(p["grad_y"]), _np(p["grad_final"]), _unit(dtype))
+    if lens is not None:
+        for k in ("x", "gate", "grad_y"):
+            _poison(p[k], lens)
+    p["lens"] = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    return p, want
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("case", RECURRENCES, ids=lambda c: "%dx%dx%d-%s" % (c[0], c[1], c[2], c[6]))
+def test_recurrence(case, dtype):
+    n, t, c, lens, reverse, with_initial, layout = case
+    p, want = _recurrence_problem(case, dtype, 7 * n + 11 * t + c)
+    leaves = []
+    if layout == "packed":
+        x, gate = torch.cat((p["x"], p["gate"]), 2).requires_grad_(True), None
+        leaves.append(x)
+    else:
+        x, gate = (_laid_out(p[k], layout).detach().requires_grad_(True) for k in ("x", "gate"))
+        leaves += [x, gate]
+    initial = p["initial"]
+    if with_initial:
+        leaves.append(initial.requires_grad_(True))
+    grad_y = _laid_out(p["grad_y"], layout)
+    runs = []
+    for _ in range(2):
+        y, final = sequence.gated_recurrence(x, gate, initial, p["lens"], reverse)
+        runs.append([y, final] + list(torch.autograd.grad([y, final], leaves, [grad_y, p["grad_final"]])))
+    assert all(torch.equal(a, b) for a, b in zip(*runs)), "two runs differ"
+    y, final, *grads = runs[0]
+    assert y.dtype == dtype and final.dtype == (torch.float64 if dtype == torch.float64 else torch.float32)
+    _close(y, want["y"], dtype, "y")
+    _close(final, want["final"], final.dtype, "final")
+    if layout == "packed":
+        grads[:1] = [grads[0][..., :c], grads[0][..., c:]]
+    _close(grads[0], want["grad_x"], dtype, "grad_x")
+    _close(grads[1], want["grad_gate"], dtype, "grad_gate")
+    if with_initial:
+        _close(grads[2], want["grad_initial"], final.dtype, "grad_initial")
+    if layout == "time-major" and n > 1 and t > 1:
+        assert y.transpose(0, 1).is_contiguous()
+    # without a graph: the same values from the call that keeps no states
+    with torch.no_grad():
+        y2, final2 = sequence.gated_recurrence(x, gate, initial, p["lens"], reverse)
+    assert torch.equal(y2, y) and torch.equal(final2, final)
+
+
+def test_recurrence_in_pieces():
+    """A stream fed in pieces with the state carried is the stream fed at once (the state is not rounded to 16 bits)."""
+    case = (3, 200, 40, None, False, True, "dense")
+    p, want = _recurrence_problem(case, torch.bfloat16, 5)
+    state, parts, at = p["initial"], [], 0
+    for size in [1, 1, 1, 16, 30, 1, 100, 50]:
+        y, state = sequence.gated_recurrence(p["x"][:, at:at + size], p["gate"][:, at:at + size], state)
+        parts.append(y)
+        at += size
+    assert at == 200
+    _close(torch.cat(parts, 1), want["y"], torch.bfloat16, "y")
+    _close(state, want["final"], torch.float32, "final")
+
+
+def test_recurrence_extreme_gates():
+    """Gates that are shut or open for good, in the type's whole range: no NaN, and exactly the kept or the new value."""
+    for dtype in TYPES:
+        top = torch.finfo(dtype).max
+        gate = torch.tensor([top, -top, float("inf"), float("-inf"), 200.0, -200.0], device="cuda", dtype=dtype)
+        gate = gate.repeat(40).view(1, -1, 1).expand(1, 240, 8).contiguous()
+        x = torch.arange(1, 241, device="cuda", dtype=dtype).view(1, -1, 1).expand(1, 240, 8).contiguous().requires_grad_(True)
+        y, final = sequence.gated_recurrence(x, gate.requires_grad_(True))
+        # odd frames take their value, even ones keep the state
+        want = torch.arange(1, 241).view(-1, 2)[:, 0] - 1
+        assert torch.equal(y[0, :, 0].double().cpu(), torch.stack((want, want + 2), 1).view(-1).to(dtype).double()), dtype
+        gx, gg = torch.autograd.grad([y.sum() + final.sum()], [x, gate])
+        # f (1 - f) <= exp(-200) = 1.4e-87 (no float32), times |h - x| and the gradient's sum, each at most 480
+        assert torch.isfinite(gx).all() and float(gg.abs().max()) <= 1e-81
+
+
+def test_recurrence_strides_beyond_32_bits():
+    """Frames 2^30 elements apart: the offsets pass 32 bits."""
+    flat = torch.zeros(5 * 2 ** 30 + 64, dtype=torch.bfloat16, device="cuda")
+    x = flat.as_strided((1, 6, 32), (0, 2 ** 30, 1))
+    gate = flat[32:].as_strided((1, 6, 32), (0, 2 ** 30, 1))
+    small = torch.randn(1, 6, 32, device="cuda").bfloat16(), torch.randn(1, 6, 32, device="cuda").bfloat16()
+    x.copy_(small[0])
+    gate.copy_(small[1])
+    got, want = sequence.gated_recurrence(x, gate), sequence.gated_recurrence(*small)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_recurrence_empty():
+    for shape in ((0, 5, 8), (2, 0, 8), (2, 5, 0)):
+        x = torch.randn(*shape, device="cuda", requires_grad=True)
+        gate = torch.randn(*shape, device="cuda", requires_grad=True)
+        initial = torch.randn(shape[0], shape[2], device="cuda", requires_grad=True)
+        y, final = sequence.gated_recurrence(x, gate, initial)
+        assert y.shape == shape and torch.equal(final, initial)
+        grads = torch.autograd.grad(y.sum() + 2 * final.sum(), [x, gate, initial])
+        assert torch.equal(grads[0], torch.zeros_like(x)) and (shape[1] or torch.equal(grads[2], torch.full_like(initial, 2)))
+
+
+def test_recurrence_gradients_of_one_output_and_broadcast():
+    """Only one output used; an expanded input, an expanded gradient."""
+    gate = torch.randn(2, 20, 8, device="cuda", dtype=torch.float64, requires_grad=True)
+    row = torch.randn(1, 1, 8, device="cuda", dtype=torch.float64, requires_grad=True)
+    for pick in (lambda y, final: y.sum(), lambda y, final: final.sum()):
+        got = torch.autograd.grad(pick(*sequence.gated_recurrence(row.expand(2, 20, 8), gate)), [row, gate])
+        full = row.detach().expand(2, 20, 8).contiguous().requires_grad_(True)
+        want = torch.autograd.grad(pick(*sequence.gated_recurrence(full, gate)), [full, gate])
+        assert torch.allclose(got[0], want[0].sum((0, 1), keepdim=True), rtol=1e-13, atol=0) and torch.equal(got[1], want[1])
+
+
+# ---- group norm with an activation -----------------------------------------------------------------------------------
+
+# (batch, frames, channels, groups, lens, activation, with parameters, layout)
+NORMS = [
+    (1, 1, 1, 1, None, "none", True, "dense"),
+    (2, 1, 64, 8, None, "relu", True, "dense"),
+    (300, 1, 96, 4, None, "silu", True, "dense"),
+    (3, 5, 12, 3, [5, 0, 1], "gelu", True, "dense"),
+    (2, 41, 256, 8, None, "relu", True, "dense"),
+    (4, 33, 66, 11, [33, 0, 32, 7], "silu", True, "odd"),
+    (2, 64, 128, 1, [40, 64], "gelu", False, "time-major"),
+    (2, 65, 128, 128, [65, 64], "none", True, "wide"),
+    (3, 130, 330, 11, [129, -1, 130], "gelu", True, "dense"),
+    (2, 200, 1024, 32, [200, 77], "relu", True, "dense"),
+    (2, 100, 72, 2, None, "silu", True, "channels apart"),
+    (1, 1500, 40, 5, [1499], "silu", True, "dense"),
+    (1, 3001, 512, 2, None, "gelu", True, "wide"),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("case", NORMS, ids=lambda c: "%dx%dx%d-%d-%s-%s" % (c[0], c[1], c[2], c[3], c[5], c[7]))
+def test_group_norm_act(case, dtype):
+    n, t, c, groups, lens, act, affine, layout = case
+    rng = np.random.default_rng(13 * n + 5 * t + c)
+    state = torch.float64 if dtype == torch.float64 else torch.float32
+    x = torch.from_numpy(rng.standard_normal((n, t, c)) * 1.5 + 0.5).to("cuda").to(dtype)
+    grad_y = torch.from_numpy(rng.standard_normal((n, t, c))).to("cuda").to(dtype)
+    weight = bias = None
+    if affine:
+        weight = torch.from_numpy(1 + 0.3 * rng.standard_normal(c)).to("cuda").to(state).requires_grad_(True)
+        bias = torch.from_numpy(0.3 * rng.standard_normal(c)).to("cuda").to(state).requires_grad_(True)
+    want = so.group_norm_act(_np(x), groups, None if weight is None else _np(weight), None if bias is None else _np(bias),
+                             lens, 1e-5, act, _np(grad_y), _unit(dtype))
+    if lens is not None:
+        _poison(x, lens), _poison(grad_y, lens)
+    x, grad_y = _laid_out(x, layout).detach().requires_grad_(True), _laid_out(grad_y, layout)
+    lens_d = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    leaves = [x] + ([weight, bias] if affine else [])
+    runs = []
+    for _ in range(2):
+        y = sequence.group_norm_act(x, groups, weight, bias, lens_d, 1e-5, act)
+        runs.append([y] + list(torch.autograd.grad(y, leaves, grad_y)))
+    assert all(torch.equal(a, b) for a, b in zip(*runs)), "two runs differ"
+    y, gx, *grads = runs[0]
+    assert y.dtype == dtype
+    _close(y, want["y"], dtype, "y")
+    _close(gx, want["grad_x"], dtype, "grad_x")
+    if affine:
+        _close(grads[0], want["grad_weight"], state, "grad_weight")
+        _close(grads[1], want["grad_bias"], state, "grad_bias")
+    with torch.no_grad():
+        assert torch.equal(sequence.group_norm_act(x, groups, weight, bias, lens_d, 1e-5, act), y)
+
+
+def test_group_norm_large_mean():
+    """Values far from zero: the variance is taken from deviations, not as a difference of squares.
+
+    x = 4096 + z in float32 is exact to 2^-12; the deviations' relative error is about 2^-12 at worst from the mean's
+    rounding (2^-12 absolute), which moves every value alike and leaves the variance at 2^-24 relative."""
+    z = torch.randn(2, 300, 64, device="cuda", dtype=torch.float64)
+    x = (z + 4096).float()
+    y = sequence.group_norm_act(x, 8, activation="none").double()
+    d = x.double().view(2, 300, 8, 8)
+    want = ((d - d.mean((1, 3), keepdim=True)) / (d.var((1, 3), unbiased=False, keepdim=True) + 1e-5).sqrt()).view_as(x)
+    assert float((y - want).abs().max()) <= 2 ** -10
+    assert abs(float(y.var(unbiased=False)) - 1) <= 1e-3
+
+
+def test_group_norm_other_shapes():
+    """(batch, channels), images channels last, 16-bit parameters, no frames, no utterances."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(5, 64, device="cuda", generator=gen)
+    assert torch.equal(sequence.group_norm_act(x, 4, activation="silu"),
+                       sequence.group_norm_act(x.view(5, 1, 64), 4, activation="silu").view(5, 64))
+    image = torch.randn(2, 32, 9, 11, device="cuda", generator=gen).to(memory_format=torch.channels_last)
+    y = sequence.group_norm_act(image.permute(0, 2, 3, 1), 4, activation="relu")
+    want = so.group_norm_act(_np(image.permute(0, 2, 3, 1).reshape(2, 99, 32)), 4, act="relu")["y"]
+    _close(y.reshape(2, 99, 32), want, torch.float32, "image")
+    w = (1 + torch.randn(64, device="cuda", generator=gen)).bfloat16().requires_grad_(True)
+    x16 = x.bfloat16().requires_grad_(True)
+    y = sequence.group_norm_act(x16, 4, w)
+    assert torch.equal(y, sequence.group_norm_act(x16, 4, w.float()))
+    gw, = torch.autograd.grad(y.sum(), [w])
+    assert gw.dtype == torch.bfloat16
+    for shape in ((0, 5, 8), (2, 0, 8)):
+        e = torch.randn(*shape, device="cuda", requires_grad=True)
+        weight, bias = torch.ones(8, device="cuda", requires_grad=True), torch.zeros(8, device="cuda", requires_grad=True)
+        y = sequence.group_norm_act(e, 2, weight, bias)
+        assert y.shape == shape
+        grads = torch.autograd.grad(y.sum(), [e, weight, bias])
+        assert all(torch.equal(g, torch.zeros_like(g)) for g in grads)
+
+
+def test_group_norm_strides_beyond_32_bits():
+    flat = torch.zeros(5 * 2 ** 30 + 64, dtype=torch.bfloat16, device="cuda")
+    x = flat.as_strided((1, 6, 32), (0, 2 ** 30, 1))
+    small = torch.randn(1, 6, 32, device="cuda").bfloat16()
+    x.copy_(small)
+    assert torch.equal(sequence.group_norm_act(x, 4), sequence.group_norm_act(small, 4))
+
+
+# ---- counter-based dropout -------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape,layout", [((1,), "dense"), ((3,), "dense"), ((1024,), "dense"), ((7, 13), "dense"),
+                                          ((2, 33, 40), "wide"), ((4, 5, 64), "time-major"), ((3, 7, 11), "odd"),
+                                          ((2, 3, 21), "wide"), ((3, 1000, 37), "dense"), ((64, 1, 512), "dense")])
+def test_dropout(shape, layout, dtype):
+    rng = np.random.default_rng(sum(shape))
+    u = _unit(dtype)
+    for p, seed, with_residual in ((0.05, 1, False), (0.5, 2 ** 63 + 12345, True), (1.0, 7, True), (0.3, -1, False)):
+        x = torch.from_numpy(rng.standard_normal(shape)).to("cuda").to(dtype)
+        grad_y = torch.from_numpy(rng.standard_normal(shape)).to("cuda").to(dtype)
+        residual = torch.from_numpy(rng.standard_normal(shape)).to("cuda").to(dtype) if with_residual else None
+        keep = so.dropout_keep(shape, p, seed & (2 ** 64 - 1))
+        # what is dropped must not be seen
+        x[torch.from_numpy(~keep).cuda()] = float("nan")
+        scale = 1 / (1 - p) if p < 1 else 0.0
+        kept = np.where(keep, np.nan_to_num(_np(x)) * scale, 0)
+        value = kept + (_np(residual) if with_residual else 0)
+        # the factor, the product and the sum are rounded once each
+        bound = 2 * u * np.abs(kept) + u * np.abs(value)
+        if len(shape) == 3:
+            x, grad_y = _laid_out(x, layout), _laid_out(grad_y, layout)
+            residual = _laid_out(residual, layout) if with_residual else None
+        x = x.detach().requires_grad_(True)
+        leaves = [x] + ([residual.requires_grad_(True)] if with_residual else [])
+        y = sequence.philox_dropout(x, p, True, seed, residual)
+        grads = torch.autograd.grad(y, leaves, grad_y)
+        assert y.dtype == dtype and y.shape == torch.Size(shape)
+        _close(y, (value, bound), dtype, "y")
+        g = np.where(keep, _np(grad_y) * scale, 0)
+        _close(grads[0], (g, 2 * u * np.abs(g)), dtype, "grad_x")
+        if with_residual:
+            assert torch.equal(grads[1], grad_y)
+        by_tensor = sequence.philox_dropout(x, p, True, torch.tensor(seed if seed < 2 ** 63 else seed - 2 ** 64, device="cuda"),
+                                            residual)
+        assert torch.equal(by_tensor, y)
+
+
+def test_dropout_evaluation_and_defaults():
+    x, r = torch.randn(4, 50, device="cuda"), torch.randn(4, 50, device="cuda")
+    assert sequence.philox_dropout(x, 0.5, False) is x and sequence.philox_dropout(x, 0.0) is x
+    assert torch.equal(sequence.philox_dropout(x, 0.5, False, residual=r), x + r)
+    torch.manual_seed(5)
+    a = sequence.philox_dropout(x, 0.5)
+    torch.manual_seed(5)
+    assert torch.equal(sequence.philox_dropout(x, 0.5), a) and not torch.equal(sequence.philox_dropout(x, 0.5), a)
+    assert sequence.philox_dropout(torch.empty(0, 4, device="cuda"), 0.5).shape == (0, 4)
+    big = torch.ones(1 << 20, device="cuda")
+    kept = float((sequence.philox_dropout(big, 0.1, True, 99) != 0).float().mean())
+    assert abs(kept - 0.9) <= 5 * (0.09 / (1 << 20)) ** 0.5
+
+
+def test_dropout_offsets_beyond_32_bits():
+    """The counter's upper half: elements from 2^34 on (counter 2^32) draw other words than those from 0 on."""
+    count = 2 ** 34 + 4096
+    x = torch.ones(1, dtype=torch.bfloat16, device="cuda").expand(count // 4096, 4096)  # one value, read at every row
+    x = x[:, :1].expand(count // 4096, 4096)
+    y = sequence.philox_dropout(torch.ones(1, 4096, dtype=torch.bfloat16, device="cuda").expand(count // 4096, 4096), 0.5, True, 11)
+    words = so.philox4x32_10(np.arange(2 ** 32, 2 ** 32 + 1024), 11).reshape(-1)
+    assert np.array_equal(_np(y[-1]) != 0, words >= 2 ** 31)
+    assert np.array_equal(_np(y[0]) != 0, so.dropout_keep((4096,), 0.5, 11))
+
+
+# ---- all of them -----------------------------------------------------------------------------------------------------
+
+
+def test_gradcheck():
+    lens = torch.tensor([6, 0, 3], dtype=torch.int32, device="cuda")
+    d = dict(device="cuda", dtype=torch.float64)
+    x, gate = torch.randn(3, 6, 4, **d).requires_grad_(True), torch.randn(3, 6, 4, **d).requires_grad_(True)
+    initial = torch.randn(3, 4, **d).requires_grad_(True)
+    for reverse in (False, True):
+        assert torch.autograd.gradcheck(lambda a, b, c: sequence.gated_recurrence(a, b, c, lens, reverse), (x, gate, initial))
+    packed = torch.randn(2, 20, 6, **d).requires_grad_(True)
+    assert torch.autograd.gradcheck(lambda a: sequence.gated_recurrence(a), (packed,))
+    w, b = torch.randn(4, **d).requires_grad_(True), torch.randn(4, **d).requires_grad_(True)
+    for act in ("none", "silu", "gelu"):
+        assert torch.autograd.gradcheck(lambda *a: sequence.group_norm_act(a[0], 2, a[1], a[2], lens, 1e-5, act), (x, w, b))
+    assert torch.autograd.gradcheck(lambda a, r: sequence.philox_dropout(a, 0.4, True, 3, r), (x, gate))
+
+
+def test_no_second_derivative():
+    x = torch.randn(2, 4, 6, device="cuda", requires_grad=True)
+    for y in (sequence.gated_recurrence(x)[0], sequence.group_norm_act(x, 2), sequence.philox_dropout(x, 0.5)):
+        g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once only"):
+            g.sum().backward()
+
+
+def test_refusals():
+    x = torch.randn(2, 4, 6, device="cuda")
+    lens = torch.tensor([1, 2], dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="batch, frames, channels"):
+        sequence.gated_recurrence(x[0])
+    with pytest.raises(RuntimeError, match="even number"):
+        sequence.gated_recurrence(x[..., :5])
+    with pytest.raises(RuntimeError, match="'gate' to have shape"):
+        sequence.gated_recurrence(x, x[..., :5])
+    with pytest.raises(RuntimeError, match="same dtype"):
+        sequence.gated_recurrence(x, x.half())
+    with pytest.raises(RuntimeError, match="'initial' to have shape"):
+        sequence.gated_recurrence(x, x, x[:, 0, :3])
+    with pytest.raises(RuntimeError, match="must be float16"):
+        sequence.gated_recurrence(x.int())
+    for bad in (lens.long(), lens.cpu(), lens[:1], lens.view(2, 1)):
+        with pytest.raises(RuntimeError, match="lens"):
+            sequence.gated_recurrence(x, lens=bad)
+        with pytest.raises(RuntimeError, match="lens"):
+            sequence.group_norm_act(x, 2, lens=bad)
+    with pytest.raises(RuntimeError, match="do not divide"):
+        sequence.group_norm_act(x, 4)
+    with pytest.raises(RuntimeError, match="do not divide"):
+        sequence.group_norm_act(x, 0)
+    with pytest.raises(RuntimeError, match="'weight' to have shape"):
+        sequence.group_norm_act(x, 2, x[0, 0, :3])
+    with pytest.raises(RuntimeError, match="eps"):
+        sequence.group_norm_act(x, 2, eps=-1.0)
+    with pytest.raises(ValueError, match="activation"):
+        sequence.group_norm_act(x, 2, activation="tanh")
+    with pytest.raises(RuntimeError, match="lens"):
+        sequence.group_norm_act(x.view(2, 2, 2, 6), 2, lens=lens)
+    with pytest.raises(ValueError, match="p must be"):
+        sequence.philox_dropout(x, -0.1)
+    with pytest.raises(RuntimeError, match="same dtype"):
+        sequence.philox_dropout(x, 0.1, residual=x.half())
+    with pytest.raises(RuntimeError, match="'residual' to have shape"):
+        sequence.philox_dropout(x, 0.1, residual=x[:1])
+    with pytest.raises(RuntimeError, match="seed tensor"):
+        sequence.philox_dropout(x, 0.1, seed=torch.zeros(2, dtype=torch.int64, device="cuda"))
+    seed = torch.tensor(3, device="cuda")
+    y = sequence.philox_dropout(x.requires_grad_(True), 0.5, seed=seed)
+    seed.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_other_stream_and_captured_graph():
+    """The same results on a stream of the caller's, and from a graph that is replayed on other inputs."""
+    lens = torch.tensor([40, 0, 25], dtype=torch.int32, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    w, b = torch.randn(32, device="cuda", generator=gen), torch.randn(32, device="cuda", generator=gen)
+    seed = torch.tensor(1, device="cuda")
+    x = torch.randn(3, 40, 64, device="cuda", generator=gen)
+
+    def step(x):
+        x = x.detach().requires_grad_(True)
+        y, final = sequence.gated_recurrence(x, lens=lens)
+        z = sequence.group_norm_act(y, 4, w, b, lens, activation="silu")
+        out = sequence.philox_dropout(z, 0.2, True, seed, y)
+        return [out, final] + list(torch.autograd.grad([out, final], [x], [torch.ones_like(out), torch.ones_like(final)]))
+
+    eager = step(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step(x)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, c) for a, c in zip(eager, other))
+    static = x.clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured = step(static)
+    for k in range(3):
+        static.copy_(x * (k + 1))
+        seed.fill_(k + 1)
+        lens.copy_(torch.tensor([40 - k, k, 25], dtype=torch.int32))
+        graph.replay()
+        want = step(x * (k + 1))
+        assert all(torch.equal(a, c) for a, c in zip(captured, want)), k
+
+
+def test_autocast_meets_in_the_wider_type():
+    x = torch.randn(2, 6, 8, device="cuda")
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert sequence.philox_dropout(x.bfloat16(), 0.5, True, 1, x).dtype == torch.float32
+        assert sequence.gated_recurrence(x.bfloat16(), x)[0].dtype == torch.float32
+        assert sequence.group_norm_act(x.bfloat16(), 2).dtype == torch.bfloat16
+
+
+def test_launches():
+    """One kernel each way for the recurrence and the dropout."""
+    x = torch.randn(2, 40, 64, device="cuda", requires_grad=True)
+    before = capi.launch_count()
+    y, _ = sequence.gated_recurrence(x)
+    assert capi.launch_count() - before == 1
+    torch.autograd.grad(y.sum(), x)
+    assert capi.launch_count() - before == 2
+    z = sequence.philox_dropout(x, 0.5)
+    assert capi.launch_count() - before == 3
+    torch.autograd.grad(z.sum(), x)
+    assert capi.launch_count() - before == 4
+    assert capi.device_status() == 0
