@@ -114,12 +114,12 @@ __global__ void __launch_bounds__(kThreads) norm_moments_kernel(const NormArgs<T
   for (int v = 0; v < V; ++v) mean[v] = m2[v] = 0;
   if (s.c < a.channels) {
     for (long long t = s.begin + ty; t < s.end; t += rows) {
-      const Pack<T, V> p = *reinterpret_cast<const Pack<T, V> *>(a.x.p + s.n * a.x.sn + t * a.x.st + s.c);
+      const Raw<T, V> p = load_raw<T, V>(a.x.p + s.n * a.x.sn + t * a.x.st + s.c);
       count += A(1);
       const A inv = A(1) / count;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const A value = to_acc(p.v[v]), delta = value - mean[v];
+        const A value = element(p, v), delta = value - mean[v];
         mean[v] += delta * inv;
         m2[v] += delta * (value - mean[v]);
       }
@@ -197,19 +197,19 @@ __global__ void __launch_bounds__(kThreads) norm_apply_kernel(const NormArgs<T> 
   ChannelParams<T, V> q;
   q.load(a, s.n, s.c);
   for (long long t = s.begin + threadIdx.x / a.tx; t < s.end; t += kThreads / a.tx) {
-    Pack<T, V> o;
+    A o[V];
     if (t < upto) {
-      const Pack<T, V> p = *reinterpret_cast<const Pack<T, V> *>(a.x.p + s.n * a.x.sn + t * a.x.st + s.c);
+      const Raw<T, V> p = load_raw<T, V>(a.x.p + s.n * a.x.sn + t * a.x.st + s.c);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const A xhat = (to_acc(p.v[v]) - q.mean[v]) * q.rstd[v];
-        o.v[v] = from_acc<T>(act_value(xhat * q.weight[v] + q.bias[v], a.act));
+        const A xhat = (element(p, v) - q.mean[v]) * q.rstd[v];
+        o[v] = act_value(xhat * q.weight[v] + q.bias[v], a.act);
       }
     } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v) o.v[v] = from_acc<T>(A(0));
+      for (int v = 0; v < V; ++v) o[v] = A(0);
     }
-    *reinterpret_cast<Pack<T, V> *>(a.y.p + s.n * a.y.sn + t * a.y.st + s.c) = o;
+    store_raw<T, V>(a.y.p + s.n * a.y.sn + t * a.y.st + s.c, rounded<T, V>(o));
   }
 }
 
@@ -227,12 +227,12 @@ __global__ void __launch_bounds__(kThreads) norm_sums_kernel(const NormArgs<T> a
     ChannelParams<T, V> q;
     q.load(a, s.n, s.c);
     for (long long t = s.begin + ty; t < s.end; t += rows) {
-      const Pack<T, V> p = *reinterpret_cast<const Pack<T, V> *>(a.x.p + s.n * a.x.sn + t * a.x.st + s.c);
-      const Pack<T, V> gy = *reinterpret_cast<const Pack<T, V> *>(a.grad_y.p + s.n * a.grad_y.sn + t * a.grad_y.st + s.c);
+      const Raw<T, V> p = load_raw<T, V>(a.x.p + s.n * a.x.sn + t * a.x.st + s.c);
+      const Raw<T, V> gy = load_raw<T, V>(a.grad_y.p + s.n * a.grad_y.sn + t * a.grad_y.st + s.c);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const A xhat = (to_acc(p.v[v]) - q.mean[v]) * q.rstd[v];
-        const A gz = to_acc(gy.v[v]) * act_slope(xhat * q.weight[v] + q.bias[v], a.act);
+        const A xhat = (element(p, v) - q.mean[v]) * q.rstd[v];
+        const A gz = element(gy, v) * act_slope(xhat * q.weight[v] + q.bias[v], a.act);
         sum[2 * v] += gz, sum[2 * v + 1] += gz * xhat;
       }
     }
@@ -298,21 +298,21 @@ __global__ void __launch_bounds__(kThreads) norm_grad_input_kernel(const NormArg
     s1[v] = in[0], s2[v] = in[1];
   }
   for (long long t = s.begin + threadIdx.x / a.tx; t < s.end; t += kThreads / a.tx) {
-    Pack<T, V> o;
+    A o[V];
     if (t < upto) {
-      const Pack<T, V> p = *reinterpret_cast<const Pack<T, V> *>(a.x.p + s.n * a.x.sn + t * a.x.st + s.c);
-      const Pack<T, V> gy = *reinterpret_cast<const Pack<T, V> *>(a.grad_y.p + s.n * a.grad_y.sn + t * a.grad_y.st + s.c);
+      const Raw<T, V> p = load_raw<T, V>(a.x.p + s.n * a.x.sn + t * a.x.st + s.c);
+      const Raw<T, V> gy = load_raw<T, V>(a.grad_y.p + s.n * a.grad_y.sn + t * a.grad_y.st + s.c);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const A xhat = (to_acc(p.v[v]) - q.mean[v]) * q.rstd[v];
-        const A gz = to_acc(gy.v[v]) * act_slope(xhat * q.weight[v] + q.bias[v], a.act);
-        o.v[v] = from_acc<T>(q.rstd[v] * (gz * q.weight[v] - s1[v] - xhat * s2[v]));
+        const A xhat = (element(p, v) - q.mean[v]) * q.rstd[v];
+        const A gz = element(gy, v) * act_slope(xhat * q.weight[v] + q.bias[v], a.act);
+        o[v] = q.rstd[v] * (gz * q.weight[v] - s1[v] - xhat * s2[v]);
       }
     } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v) o.v[v] = from_acc<T>(A(0));
+      for (int v = 0; v < V; ++v) o[v] = A(0);
     }
-    *reinterpret_cast<Pack<T, V> *>(a.grad_x.p + s.n * a.grad_x.sn + t * a.grad_x.st + s.c) = o;
+    store_raw<T, V>(a.grad_x.p + s.n * a.grad_x.sn + t * a.grad_x.st + s.c, rounded<T, V>(o));
   }
 }
 

@@ -37,7 +37,7 @@ __device__ __forceinline__ Words philox4x32_10(unsigned long long counter, unsig
 
 template <typename T>
 struct DropoutArgs {
-  const T *x = nullptr, *residual = nullptr;
+  const T *x = nullptr, *residual = nullptr;  // residual may be null
   T *y = nullptr;
   long long rows = 0, cols = 0, x_stride = 0, r_stride = 0;  // y is dense; strides between rows, in elements
   unsigned long long threshold = 0;                          // dropped where word < threshold; 2^32: all are
@@ -46,47 +46,64 @@ struct DropoutArgs {
   const long long *seed_device = nullptr;  // read instead of `seed` when there is one
 };
 
-// V elements a thread and turn, V a multiple of 4.  ROWS: x or the residual has rows that are not adjacent.  VEC: packed
-// accesses (everything 16-byte aligned, rows a multiple of V long); otherwise element by element.
-template <typename T, int V, bool VEC>
+// V elements a group, a multiple of 4; U groups a thread, kThreads groups apart, whose loads are issued together.  VEC:
+// whole groups by packed accesses (aligned; one row of any length, or rows a multiple of V long); the group that ends a
+// row which is no multiple of V, and everything without VEC, element by element.
+template <typename T, int V, int U, bool VEC>
 __global__ void __launch_bounds__(kThreads) philox_dropout_kernel(const DropoutArgs<T> a) {
   using A = Acc<T>;
   const unsigned long long key = a.seed_device != nullptr ? (unsigned long long)*a.seed_device : a.seed;
-  const long long total = a.rows * a.cols, groups = (total + V - 1) / V, step = (long long)gridDim.x * kThreads;
-  for (long long g = blockIdx.x * (long long)kThreads + threadIdx.x; g < groups; g += step) {
-    const long long i = g * V;
-    Pack<T, V> x, r, o;
-    if constexpr (VEC) {
-      const long long row = a.rows == 1 ? 0 : i / a.cols, col = i - row * a.cols;
-      x = *reinterpret_cast<const Pack<T, V> *>(a.x + row * a.x_stride + col);
-      if (a.residual != nullptr) r = *reinterpret_cast<const Pack<T, V> *>(a.residual + row * a.r_stride + col);
+  const long long total = a.rows * a.cols;
+  const long long first = (blockIdx.x * (long long)(kThreads * U) + threadIdx.x) * V;
+  Raw<T, V> xr[U], rr[U];
+  if constexpr (VEC) {
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      const long long i = first + (long long)q * (kThreads * V);
+      xr[q] = rr[q] = zeros<T, V>();
+      if (i + V <= total) {
+        const long long row = a.rows == 1 ? 0 : i / a.cols, col = i - row * a.cols;
+        xr[q] = load_raw<T, V>(a.x + row * a.x_stride + col);
+        if (a.residual != nullptr) rr[q] = load_raw<T, V>(a.residual + row * a.r_stride + col);
+      }
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < U; ++q) {
+    const long long i = first + (long long)q * (kThreads * V);
+    if (i >= total) return;
+    A x[V], r[V];
+    const bool whole = VEC && i + V <= total;
+    if (whole) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[v] = element(xr[q], v), r[v] = element(rr[q], v);
     } else {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
+        x[v] = r[v] = A(0);
         if (i + v < total) {
           const long long row = a.rows == 1 ? 0 : (i + v) / a.cols, col = i + v - row * a.cols;
-          x.v[v] = a.x[row * a.x_stride + col];
-          if (a.residual != nullptr) r.v[v] = a.residual[row * a.r_stride + col];
+          x[v] = to_acc(a.x[row * a.x_stride + col]);
+          if (a.residual != nullptr) r[v] = to_acc(a.residual[row * a.r_stride + col]);
         }
       }
     }
 #pragma unroll
-    for (int q = 0; q < V / 4; ++q) {
-      const Words w = philox4x32_10((unsigned long long)(i / 4 + q), key);
+    for (int g = 0; g < V / 4; ++g) {
+      const Words w = philox4x32_10((unsigned long long)(i / 4 + g), key);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int v = q * 4 + j;
-        A value = w.w[j] >= a.threshold ? to_acc(x.v[v]) * a.scale : A(0);
-        if (a.residual != nullptr) value += to_acc(r.v[v]);
-        o.v[v] = from_acc<T>(value);
+        const int v = g * 4 + j;
+        x[v] = w.w[j] >= a.threshold ? x[v] * a.scale : A(0);
+        if (a.residual != nullptr) x[v] += r[v];
       }
     }
-    if constexpr (VEC) {
-      *reinterpret_cast<Pack<T, V> *>(a.y + i) = o;
+    if (whole) {
+      store_raw<T, V>(a.y + i, rounded<T, V>(x));
     } else {
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (i + v < total) a.y[i + v] = o.v[v];
+        if (i + v < total) a.y[i + v] = from_acc<T>(x[v]);
     }
   }
 }
@@ -105,15 +122,15 @@ int run(DropoutArgs<T> a, double p, void *stream) {
     a.threshold = (unsigned long long)std::floor(p * 4294967296.0 + 0.5);
     a.scale = p < 1.0 ? (Acc<T>)(1.0 / (1.0 - p)) : Acc<T>(0);
     if (a.x_stride == a.cols && (a.residual == nullptr || a.r_stride == a.cols)) a.cols = total, a.rows = 1;
-    constexpr int V = sizeof(T) == 2 ? 8 : 4;
-    constexpr size_t bytes = sizeof(T) * V;
-    const bool vec = a.cols % V == 0 && aligned_to(a.x, bytes) && aligned_to(a.y, bytes) && aligned_to(a.residual, bytes) &&
-                     (a.rows == 1 || (a.x_stride % V == 0 && (a.residual == nullptr || a.r_stride % V == 0)));
-    const long long blocks = (total + (long long)V * kThreads - 1) / ((long long)V * kThreads);
-    const unsigned grid = (unsigned)std::min<long long>(blocks, 0x7fffffffLL);
+    constexpr int V = sizeof(T) == 2 ? 8 : 4, U = 2;
+    constexpr size_t bytes = sizeof(T) == 8 ? 16 : sizeof(T) * V;
+    const bool vec = aligned_to(a.x, bytes) && aligned_to(a.y, bytes) && aligned_to(a.residual, bytes) &&
+                     (a.rows == 1 || (a.cols % V == 0 && a.x_stride % V == 0 && a.r_stride % V == 0));
+    const long long per_block = (long long)V * U * kThreads, blocks = (total + per_block - 1) / per_block;
+    if (blocks > 0x7fffffffLL) return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": more than 2^42 elements");
     auto st = static_cast<cudaStream_t>(stream);
-    if (vec) philox_dropout_kernel<T, V, true><<<grid, kThreads, 0, st>>>(a);
-    else philox_dropout_kernel<T, V, false><<<grid, kThreads, 0, st>>>(a);
+    if (vec) philox_dropout_kernel<T, V, U, true><<<(unsigned)blocks, kThreads, 0, st>>>(a);
+    else philox_dropout_kernel<T, V, U, false><<<(unsigned)blocks, kThreads, 0, st>>>(a);
     return launched(who);
   });
 }

@@ -8,6 +8,7 @@
 #include <cstdint>
 #include <exception>
 #include <string>
+#include <type_traits>
 
 #include "../../include/mellin_b200.h"
 #include "mellin_internal.h"
@@ -45,13 +46,118 @@ __device__ __forceinline__ __nv_bfloat16 from_acc<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// V consecutive elements moved by one access; the address is a multiple of the pack's size.
+inline bool aligned_to(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
+
+// V consecutive elements as the 32-bit words they lie in, moved by accesses of up to 16 bytes (one address, a multiple of
+// the access); elements are taken out of the words only where they are used, so that loads can stay in flight.
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Pack {
-  T v[V];
+struct Raw {
+  static constexpr int kBytes = (int)sizeof(T) * V, kWords = kBytes < 4 ? 1 : kBytes / 4;
+  unsigned w[kWords];
 };
 
-inline bool aligned_to(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> load_raw(const T *p) {
+  Raw<T, V> r;
+  constexpr int BYTES = Raw<T, V>::kBytes;
+  if constexpr (BYTES == 2) {
+    r.w[0] = __ldg(reinterpret_cast<const unsigned short *>(p));
+  } else if constexpr (BYTES == 4) {
+    r.w[0] = __ldg(reinterpret_cast<const unsigned *>(p));
+  } else if constexpr (BYTES == 8) {
+    const uint2 q = __ldg(reinterpret_cast<const uint2 *>(p));
+    r.w[0] = q.x, r.w[1] = q.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+      r.w[4 * i] = q.x, r.w[4 * i + 1] = q.y, r.w[4 * i + 2] = q.z, r.w[4 * i + 3] = q.w;
+    }
+  }
+  return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_raw(T *p, const Raw<T, V> &r) {
+  constexpr int BYTES = Raw<T, V>::kBytes;
+  if constexpr (BYTES == 2) {
+    *reinterpret_cast<unsigned short *>(p) = (unsigned short)r.w[0];
+  } else if constexpr (BYTES == 4) {
+    *reinterpret_cast<unsigned *>(p) = r.w[0];
+  } else if constexpr (BYTES == 8) {
+    *reinterpret_cast<uint2 *>(p) = make_uint2(r.w[0], r.w[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i)
+      reinterpret_cast<uint4 *>(p)[i] = make_uint4(r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]);
+  }
+}
+
+// element v in the accumulation type
+template <int V>
+__device__ __forceinline__ float element(const Raw<float, V> &r, int v) {
+  return __uint_as_float(r.w[v]);
+}
+template <int V>
+__device__ __forceinline__ double element(const Raw<double, V> &r, int v) {
+  return __hiloint2double((int)r.w[2 * v + 1], (int)r.w[2 * v]);
+}
+template <int V>
+__device__ __forceinline__ float element(const Raw<__nv_bfloat16, V> &r, int v) {
+  return __uint_as_float(v & 1 ? r.w[v / 2] & 0xffff0000u : r.w[v / 2] << 16);
+}
+template <int V>
+__device__ __forceinline__ float element(const Raw<__half, V> &r, int v) {
+  return __half2float(__ushort_as_half((unsigned short)(v & 1 ? r.w[v / 2] >> 16 : r.w[v / 2])));
+}
+
+// V values rounded to T
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> rounded(const Acc<T> (&a)[V]) {
+  Raw<T, V> r;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) r.w[v] = __float_as_uint(a[v]);
+  } else if constexpr (sizeof(T) == 8) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) r.w[2 * v] = (unsigned)__double2loint(a[v]), r.w[2 * v + 1] = (unsigned)__double2hiint(a[v]);
+  } else if constexpr (V == 1) {
+    if constexpr (std::is_same<T, __half>::value) r.w[0] = __half_as_ushort(__float2half_rn(a[0]));
+    else r.w[0] = __bfloat16_as_ushort(__float2bfloat16_rn(a[0]));
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; v += 2) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 q = __floats2half2_rn(a[v], a[v + 1]);
+        r.w[v / 2] = *reinterpret_cast<const unsigned *>(&q);
+      } else {
+        const __nv_bfloat162 q = __floats2bfloat162_rn(a[v], a[v + 1]);
+        r.w[v / 2] = *reinterpret_cast<const unsigned *>(&q);
+      }
+    }
+  }
+  return r;
+}
+
+// the same value V times, as bits
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> zeros() {
+  Raw<T, V> r;
+#pragma unroll
+  for (int i = 0; i < Raw<T, V>::kWords; ++i) r.w[i] = 0;
+  return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> infinities() {
+  Raw<T, V> r;
+#pragma unroll
+  for (int i = 0; i < Raw<T, V>::kWords; ++i) {
+    if constexpr (sizeof(T) == 8) r.w[i] = i & 1 ? 0x7ff00000u : 0u;
+    else if constexpr (sizeof(T) == 4) r.w[i] = 0x7f800000u;
+    else if constexpr (std::is_same<T, __half>::value) r.w[i] = 0x7c007c00u;
+    else r.w[i] = 0x7f807f80u;
+  }
+  return r;
+}
 
 // A (batch, frames, channels) tensor whose channels are adjacent; the other two strides are free.
 template <typename T>
@@ -61,18 +167,33 @@ struct Frames {
 };
 
 // frames of utterance n that exist: lens[n] held inside [0, frames]; all of them without lens
-__device__ __forceinline__ long long live_frames(const int *lens, long long n, long long frames) {
+__device__ __forceinline__ int live_frames(const int *lens, long long n, int frames) {
   if (lens == nullptr) return frames;
-  const long long v = lens[n];
+  const int v = lens[n];
   return v < 0 ? 0 : (v > frames ? frames : v);
 }
 
-// sigmoid(g) and 1 - sigmoid(g), each to a few units in its own last place: the exponential never overflows, and the
-// complement is not formed by a subtraction
+// 2^v and 1 / v by the special function unit alone, without the scaling around it that results below 2^-126 need
+__device__ __forceinline__ float exp2_unit(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_unit(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// sigmoid(g) and 1 - sigmoid(g), each to a few units in its own last place: the complement is e sigmoid(g) with
+// e = exp(-g), not a difference.  e is held at 2^126, so that the quotient stays a normal number (the least sigmoid is
+// 2^-126); NaN stays NaN.
 __device__ __forceinline__ void sigmoid_pair(float g, float &f, float &keep) {
-  const float e = __expf(-fabsf(g)), r = __fdividef(1.f, 1.f + e), q = e * r;
-  f = g < 0.f ? q : r;
-  keep = g < 0.f ? r : q;
+  float t;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(t) : "f"(g * -1.4426950408889634f), "f"(126.f));
+  const float e = exp2_unit(t);
+  f = reciprocal_unit(1.f + e);
+  keep = e * f;
 }
 __device__ __forceinline__ void sigmoid_pair(double g, double &f, double &keep) {
   const double e = exp(-fabs(g)), r = 1.0 / (1.0 + e), q = e * r;
@@ -99,12 +220,12 @@ inline int launched(const char *who) {
   return MELLIN_OK;
 }
 
-// Extents of a (batch, frames, channels) tensor the kernels index: non-negative, the product below 2^62, each below
-// 2^31 (coordinates are 32-bit, offsets 64-bit).
+// Extents of a (batch, frames, channels) tensor the kernels index: non-negative, the product below 2^62, batch and
+// channels below 2^31, frames at most 2^30 (coordinates are 32-bit, a step past the end included; offsets are 64-bit).
 inline int check_extents(const char *who, int64_t batch, int64_t frames, int64_t channels) {
   if (batch < 0 || frames < 0 || channels < 0) return fail(MELLIN_ERR_BAD_ARGUMENT, std::string(who) + ": negative extent");
-  if (batch > 0x7fffffffLL || frames > 0x7fffffffLL || channels > 0x7fffffffLL)
-    return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": extent above 2^31 - 1");
+  if (batch > 0x7fffffffLL || frames > 0x40000000LL || channels > 0x7fffffffLL)
+    return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": batch or channels above 2^31 - 1, or frames above 2^30");
   if ((long double)batch * (long double)frames * (long double)channels > 4.0e18L)
     return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": more than 2^62 elements");
   return MELLIN_OK;
