@@ -10,9 +10,12 @@
 //   gx = rstd * (weight gz - (sum_c weight P1 + xhat * sum_c weight P2) / M)
 //
 // All sums in a fixed order: two runs give the same bits.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "sequence_common.cuh"
+#include "tc_ptx.cuh"
 
 namespace mellin {
 namespace {
@@ -20,6 +23,7 @@ namespace {
 using namespace seq;
 
 constexpr int kThreads = 256;
+constexpr int kMaxRanks = 8;    // blocks of a cluster: the portable limit
 constexpr int kMaxChunks = 64;  // pieces of an utterance's frames in the kernels that pass over the tensor twice
 
 enum Activation { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3 };
@@ -29,9 +33,20 @@ __device__ __forceinline__ double exp_of(double v) { return exp(v); }
 __device__ __forceinline__ float erf_of(float v) { return erff(v); }
 __device__ __forceinline__ double erf_of(double v) { return erf(v); }
 
+template <int ACT>
+using ActTag = std::integral_constant<int, ACT>;
+// calls body(ActTag<act>): what depends on the activation is compiled once for each
+template <typename F>
+__device__ __forceinline__ void by_act(int act, F &&body) {
+  if (act == kRelu) body(ActTag<kRelu>{});
+  else if (act == kSilu) body(ActTag<kSilu>{});
+  else if (act == kGelu) body(ActTag<kGelu>{});
+  else body(ActTag<kNone>{});
+}
+
 template <typename A>
 __device__ __forceinline__ A act_value(A z, int act) {
-  if (act == kRelu) return z > A(0) ? z : (z <= A(0) ? A(0) : z);  // NaN stays
+  if (act == kRelu) return max_nan(z, A(0));
   if (act == kSilu) {
     A f, keep;
     sigmoid_pair(z, f, keep);
@@ -65,12 +80,365 @@ struct NormArgs {
   const int *lens = nullptr;
   int batch = 0, frames = 0, channels = 0, groups = 0, act = 0;
   Acc<T> eps = 0;
+  // the fused kernels
+  int team = 0, col_ranks = 1, row_ranks = 1;  // threads that share a group in a block; blocks of a cluster across both
+  int team_log2 = 0, across = 1, packs = 1, rows = 1;  // blocks across the groups, packs of a frame, frames of a team
+  unsigned packs_magic = 0;                            // ceil(2^20 / packs)
+  int kept = 0;                                // most frames of a thread in shared memory
+  int per_block = 1;                           // utterances a backward block takes one after the other
+  int parts = 1;                               // sets of parameter sums: (parts, channels, 2) at `part`
   // the kernels that pass over the tensor twice
   Acc<T> *part = nullptr;    // (batch, chunks, channels, 2)
   Acc<T> *sums = nullptr;    // (batch, channels, 2): P1, P2
   Acc<T> *gsums = nullptr;   // (batch, groups, 2): sums of weight * P1, weight * P2, over M
   int chunks = 0, tx = 0, slabs = 0;
 };
+
+// (mean, sum of squared deviations, count) of two sets of values, joined
+template <typename A>
+__device__ __forceinline__ void join(A &mean, A &m2, A &count, A mean_b, A m2_b, A count_b) {
+  if (count_b == A(0)) return;
+  const A total = count + count_b, delta = mean_b - mean, share = count_b * reciprocal_unit(total);
+  mean += delta * share;
+  m2 += m2_b + delta * delta * count * share;
+  count = total;
+}
+
+// ---- one pass: a group's values stay in shared memory between the sums and the result ---------------------------------
+//
+// `team` threads of a block (or the blocks of a cluster, team = all threads of each) share one utterance's group.  A
+// thread has V adjacent channels, always the same, of every `rows`-th frame; the first `kept` of its frames are copied
+// to its own slots in shared memory, all copies issued at once, so x (and grad_y) is read from HBM once.  Frames beyond
+// those are read again for the result, from L2 as a rule.  Teams are as small as the group allows, down to four threads,
+// so that groups of a single frame share a warp.  Bound by HBM: two or more blocks a multiprocessor overlap one's sums
+// with another's loads and stores.  (Kept in registers instead, 64 a thread, float32 at 32 x 200..800 x
+// 1024 took 68 us forward and 151 us backward against 39 and 61: fewer bytes in flight, more clusters, code beyond the
+// instruction cache.)
+
+struct Seat {  // a thread's place
+  int n, len, g, c, rank, size, team_id, j, tx, ty, rows, row_rank, cols;
+  bool some, live;  // there are columns for this rank; this thread has one
+};
+template <typename T, int V>
+__device__ __forceinline__ Seat seat_of(const NormArgs<T> &a, bool sorted) {
+  Seat s;
+  s.size = a.col_ranks * a.row_ranks, s.rank = 0;
+  unsigned block = blockIdx.x, col_rank = 0;
+  s.row_rank = 0;
+  if (s.size > 1) {
+    s.rank = (int)(block % (unsigned)s.size), block /= (unsigned)s.size;
+    s.row_rank = s.rank, col_rank = 0;
+    if (a.col_ranks > 1) s.row_rank = s.rank / a.col_ranks, col_rank = (unsigned)s.rank % a.col_ranks;
+  }
+  const unsigned turn = a.across == 1 ? block : block / (unsigned)a.across;
+  if (sorted) {
+    const Utterance u = utterance_of(a.lens, a.batch, a.frames, (int)turn);
+    s.n = u.n, s.len = u.len;
+  } else {
+    s.n = (int)turn, s.len = 0;
+  }
+  s.team_id = (int)(threadIdx.x >> a.team_log2), s.j = (int)(threadIdx.x & ((1u << a.team_log2) - 1));
+  s.g = (int)((block - turn * a.across) * (kThreads >> a.team_log2)) + s.team_id;
+  s.cols = a.packs, s.rows = a.rows, s.some = true;
+  if (a.col_ranks > 1) {
+    const int left = a.packs - (int)col_rank * a.team;  // none for the last ranks where the ranks are not a multiple
+    s.some = left > 0;
+    s.cols = left < 1 ? 1 : (left < a.team ? left : a.team);
+    s.rows = a.team / s.cols;
+    s.ty = s.j / s.cols;
+  } else {
+    s.ty = (int)((unsigned)s.j * a.packs_magic >> 20);  // j / packs, exact for j and packs up to 512
+  }
+  s.tx = s.j - s.ty * s.cols;
+  s.live = s.g < a.groups && s.ty < s.rows && s.some;
+  s.c = (s.g * a.packs + (int)col_rank * a.team + s.tx) * V;
+  return s;
+}
+struct Span {
+  int begin, end;
+};
+__device__ __forceinline__ Span span_of(int len, int rank, int ranks) {
+  if (ranks == 1) return {0, len};
+  const int rows = (int)((unsigned)(len + ranks - 1) / (unsigned)ranks);
+  const long long begin = (long long)rows * rank;
+  Span s;
+  s.begin = begin < len ? (int)begin : len;
+  s.end = len - s.begin < rows ? len : s.begin + rows;
+  return s;
+}
+
+// Zeros in the frames first, first + step, ... behind an utterance's end
+template <typename T, int V>
+__device__ __forceinline__ void clear_from(const Frames<T> &f, long long n, int c, int first, int step, int frames) {
+  T *p = f.p + n * f.sn + first * f.st + c;
+  const long long jump = step * f.st;
+  for (int t = first; t < frames; t += step, p += jump) store_raw<T, V>(p, zeros<T, V>());
+}
+
+// count, mean and sum of squared deviations of a thread's values, taken in a few frames at a time relative to the first of
+// them: a pivot that is one of n values costs the squares at most n units in the last place
+template <typename A>
+struct Moments {
+  A mean = 0, m2 = 0, count = 0;
+};
+constexpr int kBatch = 16;  // frames a thread takes into its moments together
+template <typename T, int V, typename F>
+__device__ __forceinline__ void add_frames(Moments<Acc<T>> &m, int frames, F &&frame) {
+  using A = Acc<T>;
+  for (int i0 = 0; i0 < frames; i0 += kBatch) {
+    A pivot = 0, sum = 0, squares = 0;
+    const int n = min(kBatch, frames - i0);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (i < n) {
+        const Raw<T, V> r = frame(i0 + i);
+        if (i == 0) pivot = element(r, 0);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const A d = element(r, v) - pivot;
+          sum += d, squares += d * d;
+        }
+      }
+    }
+    const A count = A(n * V), off = sum * reciprocal_unit(count);
+    join(m.mean, m.m2, m.count, pivot + off, max(squares - sum * off, A(0)), count);
+  }
+}
+
+// A cluster's barrier in two halves: what lies between them does not wait for blocks that have not started
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
+// Sum over a team, the same bits in all its threads; `slots` (one a warp) is not used again before the next block barrier
+// but one.
+template <typename A>
+__device__ __forceinline__ A team_sum(A v, const Seat &s, int team, A *slots) {
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const A other = __shfl_xor_sync(0xffffffffu, v, o);
+    if (o < team) v += other;
+  }
+  if (team > 32) {
+    if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+    __syncthreads();
+    if (team == kThreads) {
+      A all[kThreads / 32];
+#pragma unroll
+      for (int i = 0; i < kThreads / 32; ++i) all[i] = slots[i];
+#pragma unroll
+      for (int o = kThreads / 64; o > 0; o /= 2)
+#pragma unroll
+        for (int i = 0; i < o; ++i) all[i] += all[i + o];
+      v = all[0];
+    } else {
+      v = 0;
+      for (int i = 0; i < team / 32; ++i) v += slots[s.team_id * (team / 32) + i];
+    }
+  }
+  return v;
+}
+
+template <typename T, int V, int MB>
+__global__ void __launch_bounds__(kThreads, MB) norm_fused_kernel(const NormArgs<T> a) {
+  using A = Acc<T>;
+  extern __shared__ __align__(16) unsigned char shared_raw[];
+  __shared__ __align__(16) A slots[2][kThreads / 32];
+  __shared__ A ranks[kMaxRanks][3];
+  const Seat s = seat_of<T, V>(a, true);
+  if (s.size > 1) cluster_arrive();
+  const int len = s.len;
+  const Span span = span_of(len, s.row_rank, a.row_ranks);
+  const int first = span.begin + s.ty, end = s.live ? span.end : 0;
+  const int frames = first < end ? (int)((unsigned)(end - first + s.rows - 1) / (unsigned)s.rows) : 0, kept = min(frames, a.kept);
+  const T *x = a.x.p + s.n * a.x.sn + first * a.x.st + s.c;
+  const long long jump = s.rows * a.x.st;
+  T *mine = reinterpret_cast<T *>(shared_raw) + threadIdx.x * V;  // frame i at mine + i * kThreads * V
+  const T *from = x;
+  for (int i = 0; i < kept; ++i, from += jump) copy_async<T, V>(mine + i * (kThreads * V), from);
+  if (s.live) clear_from<T, V>(a.y, s.n, s.c, len + s.row_rank * s.rows + s.ty, a.row_ranks * s.rows, a.frames);
+  A scale[V], shift[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    scale[v] = a.weight != nullptr && s.live ? a.weight[s.c + v] : A(1);
+    shift[v] = a.bias != nullptr && s.live ? a.bias[s.c + v] : A(0);
+  }
+  Moments<A> m;
+  if (frames > kept) add_frames<T, V>(m, frames - kept, [&](int i) { return load_raw<T, V>(x + (kept + i) * jump); });
+  copies_done();
+  add_frames<T, V>(m, kept, [&](int i) { return load_shared<T, V>(mine + i * (kThreads * V)); });
+
+  // the block's: sum of the values, then of the squared deviations from their mean
+  A count = A(span.end - span.begin) * A(s.some ? s.cols * V : 0);
+  const A total = team_sum<A>(m.count * m.mean, s, a.team, slots[0]);
+  A mean = count > A(0) ? total / count : A(0);
+  const A d = m.mean - mean;
+  A m2 = team_sum<A>(m.m2 + m.count * d * d, s, a.team, slots[1]);
+  if (s.size > 1) {
+    auto cluster = cooperative_groups::this_cluster();
+    cluster_wait();  // no block writes to one that has not started
+    if (threadIdx.x < s.size) {
+      A *to = cluster.map_shared_rank(&ranks[s.rank][0], threadIdx.x);
+      to[0] = mean, to[1] = m2, to[2] = count;
+    }
+    cluster.sync();
+    mean = ranks[0][0], m2 = ranks[0][1], count = ranks[0][2];
+    for (int i = 1; i < s.size; ++i) join(mean, m2, count, ranks[i][0], ranks[i][1], ranks[i][2]);
+  }
+  if (!s.live) return;
+  const A rstd = A(1) / sqrt((count > A(0) ? m2 / count : A(0)) + a.eps);
+  if (a.stats_out != nullptr && s.j == 0 && s.rank == 0) {
+    A *out = a.stats_out + (s.n * a.groups + s.g) * 2;
+    out[0] = mean, out[1] = rstd;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) scale[v] *= rstd;
+  T *y = a.y.p + s.n * a.y.sn + first * a.y.st + s.c;
+  const long long leap = s.rows * a.y.st;
+  by_act(a.act, [&](auto act) {
+    auto result = [&](const Raw<T, V> &r, int i) {
+      A o[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) o[v] = act_value((element(r, v) - mean) * scale[v] + shift[v], decltype(act)::value);
+      store_raw<T, V>(y + i * leap, rounded<T, V>(o));
+    };
+#pragma unroll 4
+    for (int i = 0; i < kept; ++i) result(load_shared<T, V>(mine + i * (kThreads * V)), i);
+#pragma unroll 4
+    for (int i = kept; i < frames; ++i) result(load_raw<T, V>(x + i * jump), i);
+  });
+}
+
+// Backward: the same seats.  MANY: a block takes `per_block` utterances, all of whose frames fit, one after the other and
+// keeps each channel's P1, P2 over all of them, so that few sets of parameter sums are left to be added (none, where one
+// block has all utterances).
+// body(x, grad_y, i) for the frames i in [from, to), which are not in shared memory: four frames' loads at a time
+template <typename T, int V, typename F>
+__device__ __forceinline__ void again(const T *x, long long jump, const T *gy, long long jump_y, int from, int to, F &&body) {
+  constexpr int U = 4;
+  x += from * jump, gy += from * jump_y;
+  for (int i0 = from; i0 < to; i0 += U, x += U * jump, gy += U * jump_y) {
+    Raw<T, V> xq[U], yq[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (i0 + i < to) xq[i] = load_raw<T, V>(x + i * jump), yq[i] = load_raw<T, V>(gy + i * jump_y);
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (i0 + i < to) body(xq[i], yq[i], i0 + i);
+  }
+}
+
+template <typename T, int V, int MB, bool MANY>
+__global__ void __launch_bounds__(kThreads, MB) norm_fused_backward_kernel(const NormArgs<T> a) {
+  using A = Acc<T>;
+  extern __shared__ __align__(16) unsigned char shared_raw[];
+  __shared__ __align__(16) A slots[2][2][kThreads / 32];
+  __shared__ A ranks[2][kMaxRanks][2];
+  const Seat s = seat_of<T, V>(a, !MANY);
+  // with one utterance a block, `chunk` is that utterance, longest first; else the first of a run in order
+  const long long chunk = s.n, n_first = MANY ? chunk * a.per_block : chunk;
+  const long long n_end = MANY ? min(n_first + a.per_block, (long long)a.batch) : n_first + 1;
+  if (s.size > 1) cluster_arrive();
+  bool met = false;
+  A weight[V], bias[V], p1[V], p2[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    weight[v] = a.weight != nullptr && s.live ? a.weight[s.c + v] : A(1);
+    bias[v] = a.bias != nullptr && s.live ? a.bias[s.c + v] : A(0);
+    p1[v] = p2[v] = 0;
+  }
+  T *mine = reinterpret_cast<T *>(shared_raw) + threadIdx.x * V, *mine_y = mine + a.kept * (kThreads * V);
+  int buffer = 0;
+  for (long long n = n_first; n < n_end; ++n, buffer ^= 1) {
+    const int len = MANY ? live_frames(a.lens, n, a.frames) : s.len;
+    const Span span = span_of(len, s.row_rank, a.row_ranks);
+    const int first = span.begin + s.ty, end = s.live ? span.end : 0;
+    const int frames = first < end ? (int)((unsigned)(end - first + s.rows - 1) / (unsigned)s.rows) : 0, kept = min(frames, a.kept);
+    const T *x = a.x.p + n * a.x.sn + first * a.x.st + s.c, *gy = a.grad_y.p + n * a.grad_y.sn + first * a.grad_y.st + s.c;
+    const long long jump = s.rows * a.x.st, jump_y = s.rows * a.grad_y.st, leap = s.rows * a.grad_x.st;
+    const T *from = x, *from_y = gy;
+    for (int i = 0; i < kept; ++i, from += jump, from_y += jump_y) {
+      copy_async<T, V>(mine + i * (kThreads * V), from);
+      copy_async<T, V>(mine_y + i * (kThreads * V), from_y);
+    }
+    if (s.live) clear_from<T, V>(a.grad_x, n, s.c, len + s.row_rank * s.rows + s.ty, a.row_ranks * s.rows, a.frames);
+    A mean = 0, rstd = 0, scale[V], q1[V], q2[V], s1 = 0, s2 = 0;
+    if (s.live) mean = a.stats[(n * a.groups + s.g) * 2], rstd = a.stats[(n * a.groups + s.g) * 2 + 1];
+#pragma unroll
+    for (int v = 0; v < V; ++v) q1[v] = q2[v] = 0, scale[v] = rstd * weight[v];
+    by_act(a.act, [&](auto act) {
+      auto add = [&](const Raw<T, V> &xq, const Raw<T, V> &yq) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const A d = element(xq, v) - mean, gz = element(yq, v) * act_slope(d * scale[v] + bias[v], decltype(act)::value);
+          q1[v] += gz, q2[v] += gz * d;
+        }
+      };
+      if constexpr (!MANY)
+        again<T, V>(x, jump, gy, jump_y, kept, frames, [&](const Raw<T, V> &xq, const Raw<T, V> &yq, int) { add(xq, yq); });
+      copies_done();
+#pragma unroll 2
+      for (int i = 0; i < kept; ++i)
+        add(load_shared<T, V>(mine + i * (kThreads * V)), load_shared<T, V>(mine_y + i * (kThreads * V)));
+    });
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      q2[v] *= rstd;  // of gz * xhat
+      if constexpr (MANY) p1[v] += q1[v], p2[v] += q2[v];
+      else p1[v] = q1[v], p2[v] = q2[v];
+      s1 += weight[v] * q1[v], s2 += weight[v] * q2[v];
+    }
+    s1 = team_sum<A>(s1, s, a.team, slots[buffer][0]), s2 = team_sum<A>(s2, s, a.team, slots[buffer][1]);
+    if (s.size > 1) {
+      auto cluster = cooperative_groups::this_cluster();
+      if (!met) cluster_wait();
+      met = true;
+      if (threadIdx.x < s.size) {
+        A *to = cluster.map_shared_rank(&ranks[buffer][s.rank][0], threadIdx.x);
+        to[0] = s1, to[1] = s2;
+      }
+      cluster.sync();
+      s1 = s2 = 0;
+      for (int i = 0; i < s.size; ++i) s1 += ranks[buffer][i][0], s2 += ranks[buffer][i][1];
+    }
+    const A count = A(len) * A(a.channels / a.groups), inv = count > A(0) ? A(1) / count : A(0);
+    s1 *= inv * rstd, s2 *= inv * rstd * rstd;  // gx = scale gz - s1 - (x - mean) s2
+    if (!s.live) continue;
+    T *gx = a.grad_x.p + n * a.grad_x.sn + first * a.grad_x.st + s.c;
+    by_act(a.act, [&](auto act) {
+      auto result = [&](const Raw<T, V> &xq, const Raw<T, V> &yq, int i) {
+        A o[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const A d = element(xq, v) - mean, gz = element(yq, v) * act_slope(d * scale[v] + bias[v], decltype(act)::value);
+          o[v] = gz * scale[v] - (d * s2 + s1);
+        }
+        store_raw<T, V>(gx + i * leap, rounded<T, V>(o));
+      };
+#pragma unroll 2
+      for (int i = 0; i < kept; ++i)
+        result(load_shared<T, V>(mine + i * (kThreads * V)), load_shared<T, V>(mine_y + i * (kThreads * V)), i);
+      if constexpr (!MANY) again<T, V>(x, jump, gy, jump_y, kept, frames, result);
+    });
+  }
+  if (a.grad_weight == nullptr && a.grad_bias == nullptr) return;
+  // every channel's sums over the threads that have it, in the order of their frames
+  __syncthreads();  // the slots of the last utterance's frames are taken for them
+  A *columns = reinterpret_cast<A *>(shared_raw);  // [2 V][kThreads]
+#pragma unroll
+  for (int v = 0; v < V; ++v) columns[2 * v * kThreads + threadIdx.x] = p1[v], columns[(2 * v + 1) * kThreads + threadIdx.x] = p2[v];
+  __syncthreads();
+  if (s.g >= a.groups || !s.some) return;
+  const int base = threadIdx.x - s.j;
+  for (int q = s.j; q < 2 * V * s.cols; q += a.team) {
+    const int v = q / s.cols, tx = q - v * s.cols, c = s.c + (tx - s.tx) * V + v / 2;
+    A sum = 0;
+#pragma unroll 8
+    for (int r = 0; r < s.rows; ++r) sum += columns[v * kThreads + base + r * s.cols + tx];
+    if (a.parts > 1) a.part[((chunk * a.row_ranks + s.row_rank) * a.channels + c) * 2 + v % 2] = sum;
+    else if (v % 2 == 0 && a.grad_bias != nullptr) a.grad_bias[c] = sum;
+    else if (v % 2 == 1 && a.grad_weight != nullptr) a.grad_weight[c] = sum;
+  }
+}
 
 // ---- any size: pass over the tensor for the sums, pass again to normalise ------------------------------------------
 
@@ -90,16 +458,6 @@ __device__ __forceinline__ ChunkSpan chunk_span(const NormArgs<T> &a, long long 
   s.end = s.begin + rows < upto ? s.begin + rows : upto;
   s.c = (slab * a.tx + (int)(threadIdx.x % a.tx)) * V;
   return s;
-}
-
-// (mean, sum of squared deviations, count) of two sets of values, joined
-template <typename A>
-__device__ __forceinline__ void join(A &mean, A &m2, A &count, A mean_b, A m2_b, A count_b) {
-  if (count_b == A(0)) return;
-  const A total = count + count_b, delta = mean_b - mean, share = count_b / total;
-  mean += delta * share;
-  m2 += m2_b + delta * delta * count * share;
-  count = total;
 }
 
 template <typename T, int V>
@@ -316,22 +674,37 @@ __global__ void __launch_bounds__(kThreads) norm_grad_input_kernel(const NormArg
   }
 }
 
-// gweight and gbias: P2 and P1 summed over the utterances, in order
+// gweight and gbias: P2 and P1 of `parts` sets added; a block has 32 channels, 8 threads each, whose sums are joined in
+// order
 template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_grad_params_kernel(const NormArgs<T> a) {
+__global__ void __launch_bounds__(kThreads) norm_grad_params_kernel(const NormArgs<T> a, const Acc<T> *sums, int parts) {
   using A = Acc<T>;
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= a.channels) return;
+  __shared__ A s1[kThreads], s2[kThreads];
+  const int c = blockIdx.x * 32 + (int)(threadIdx.x & 31);
   A p1 = 0, p2 = 0;
-  for (long long n = 0; n < a.batch; ++n) {
-    const A *in = a.sums + (n * a.channels + c) * 2;
-    p1 += in[0], p2 += in[1];
+  tc::grid_dependency_wait();
+  if (c < a.channels) {
+#pragma unroll 4
+    for (long long n = threadIdx.x >> 5; n < parts; n += kThreads / 32) {
+      const A *in = sums + (n * a.channels + c) * 2;
+      p1 += in[0], p2 += in[1];
+    }
   }
+  s1[threadIdx.x] = p1, s2[threadIdx.x] = p2;
+  __syncthreads();
+  if (threadIdx.x >= 32 || c >= a.channels) return;
+  for (int i = 1; i < kThreads / 32; ++i) p1 += s1[i * 32 + threadIdx.x], p2 += s2[i * 32 + threadIdx.x];
   if (a.grad_weight != nullptr) a.grad_weight[c] = p2;
   if (a.grad_bias != nullptr) a.grad_bias[c] = p1;
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
+
+
+// Shared memory of a fused kernel's block: two fit a multiprocessor, or three of a forward call in 16 bits (32 utterances
+// of 200 to 800 frames, 1024 channels, 32 groups, SiLU: 27 us against 31; float32 would need twice the clusters, 45
+// against 39, and so would backward)
+constexpr int kept_bytes(int tensors, size_t element) { return (tensors == 1 && element == 2 ? 72 : 108) * 1024; }
 
 int chunks_for(int64_t batch, int64_t frames, int64_t channels) {
   // enough blocks to fill the device a few times over, at least 32 frames in each
@@ -340,19 +713,75 @@ int chunks_for(int64_t batch, int64_t frames, int64_t channels) {
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, (frames + 31) / 32, (int64_t)kMaxChunks}));
 }
 
-// workspace in elements of the accumulation type: partial sums, then (batch, channels, 2), then (batch, groups, 2)
-size_t workspace_elements(int64_t batch, int64_t frames, int64_t channels) {
-  if (batch <= 0 || frames < 0 || channels <= 0) return 0;
-  return (size_t)batch * (size_t)channels * 2 * ((size_t)chunks_for(batch, frames, channels) + 2);
-}
-
+// Elements a thread moves at once: a power of two that divides a group's channels, so that they share its statistics
 template <typename T>
 int vector_width(const NormArgs<T> &a) {
-  constexpr int V = 16 / sizeof(T);
-  auto ok = [&](const auto &f) {
-    return f.p == nullptr || (aligned_to(f.p, 16) && f.sn % V == 0 && f.st % V == 0);
+  auto ok = [](const auto &f, int V) {
+    return f.p == nullptr || (aligned_to(f.p, V * sizeof(T)) && f.sn % V == 0 && f.st % V == 0);
   };
-  return a.channels % V == 0 && ok(a.x) && ok(a.grad_y) && ok(a.y) && ok(a.grad_x) ? V : 1;
+  for (int V : {16 / (int)sizeof(T), 2})
+    if (a.channels / a.groups % V == 0 && ok(a.x, V) && ok(a.grad_y, V) && ok(a.y, V) && ok(a.grad_x, V)) return V;
+  return 1;
+}
+
+struct FusedPlan {
+  bool use = false, fits = false;  // every frame is kept
+  int team = 0, col_ranks = 1, row_ranks = 1, kept = 0;
+  long long blocks_per_utterance = 0;
+};
+
+// The fused kernels' division of a group of `per` channels, V at a time, keeping `tensors` tensors (1 forward, 2 backward)
+FusedPlan plan_fused(int64_t batch, int64_t frames, int64_t groups, int64_t per, int V, int tensors, size_t element) {
+  const int most = kept_bytes(tensors, element) / (int)(kThreads * V * element * tensors);  // frames a thread can keep
+  FusedPlan p;
+  const int64_t packs = per / V;
+  p.team = 4;
+  while (p.team < kThreads && (p.team < packs || (frames + p.team / packs - 1) / (p.team / packs) > 8)) p.team *= 2;
+  while (p.col_ranks * (int64_t)p.team < packs && p.col_ranks < kMaxRanks) p.col_ranks *= 2;
+  if (p.col_ranks * (int64_t)p.team < packs) return p;
+  const int64_t rows = std::max<int64_t>(1, p.team / packs);
+  auto kept = [&] { return ((frames + p.row_ranks - 1) / p.row_ranks + rows - 1) / rows; };
+  while (p.team == kThreads && p.col_ranks * p.row_ranks < kMaxRanks && kept() > most) p.row_ranks *= 2;
+  p.kept = (int)std::min<int64_t>(kept(), most), p.fits = kept() <= most;
+  const int teams = kThreads / p.team;
+  p.blocks_per_utterance = (groups + teams - 1) / teams * p.col_ranks * p.row_ranks;
+  // a few groups far larger than a cluster's registers: too few blocks to reach the memory's rate
+  p.use = kept() <= 2 * most || batch * p.blocks_per_utterance >= 128;
+  return p;
+}
+
+// Whether some alignment of the tensors leaves the shape to the kernels that pass over it twice
+bool may_pass_twice(int64_t batch, int64_t frames, int64_t groups, int64_t per, size_t element) {
+  for (int V : {1, 2, 4, 8})
+    if (per % V == 0 && !(plan_fused(batch, frames, groups, per, V, 1, element).use &&
+                          plan_fused(batch, frames, groups, per, V, 2, element).use))
+      return true;
+  return false;
+}
+
+// Utterances a backward block takes: all of them where that is little (one launch less), one where that leaves few sets
+// of parameter sums, else as many as leave about three rounds of two blocks a multiprocessor
+int64_t utterances_a_block(int64_t batch, int64_t frames, int64_t channels, const FusedPlan &p, size_t element) {
+  if (!p.fits) return 1;
+  if (batch <= 8 && (size_t)(frames * channels) * element <= (512u << 10)) return batch;
+  if (batch * p.row_ranks <= 512) return 1;
+  return std::max<int64_t>(1, batch * p.blocks_per_utterance / (148 * 6));
+}
+
+// workspace in elements of the accumulation type.  The fused kernels need the sets of parameter sums only; the others (batch, chunks, channels, 2), (batch, channels, 2) and (batch, groups, 2).
+size_t workspace_elements(int64_t batch, int64_t frames, int64_t channels, int64_t groups, size_t element) {
+  if (batch <= 0 || frames < 0 || channels <= 0 || groups <= 0 || channels % groups != 0) return 0;
+  size_t need = 0;
+  for (int V : {1, 2, 4, 8}) {
+    if (channels / groups % V != 0) continue;
+    const FusedPlan p = plan_fused(batch, frames, groups, channels / groups, V, 2, element);
+    if (!p.use) continue;
+    const int64_t each = utterances_a_block(batch, frames, channels, p, element);
+    need = std::max(need, (size_t)((batch + each - 1) / each) * p.row_ranks * (size_t)channels * 2);
+  }
+  if (may_pass_twice(batch, frames, groups, channels / groups, element))
+    need = std::max(need, (size_t)batch * (size_t)channels * 2 * ((size_t)chunks_for(batch, frames, channels) + 2));
+  return need;
 }
 
 template <typename T>
@@ -363,20 +792,23 @@ int prepare(const char *who, NormArgs<T> &a, int64_t batch, int64_t frames, int6
   if (groups <= 0 || channels % groups != 0)
     return fail(MELLIN_ERR_BAD_ARGUMENT, std::string(who) + ": the channels are not a multiple of the groups");
   if (act < kNone || act > kGelu) return fail(MELLIN_ERR_BAD_ARGUMENT, std::string(who) + ": unknown activation");
-  if (batch * (groups > channels ? groups : channels) > 0x7fffffffLL)
+  if (batch * std::max(groups, channels) > 0x7fffffffLL)
     return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many utterances times channels");
   a.batch = (int)batch, a.frames = (int)frames, a.channels = (int)channels, a.groups = (int)groups, a.act = act;
   if (batch == 0 || channels == 0) return MELLIN_OK;
-  const size_t need = workspace_elements(batch, frames, channels) * sizeof(Acc<T>);
-  if (workspace == nullptr || workspace_bytes < need)
+  const size_t need = workspace_elements(batch, frames, channels, groups, sizeof(T)) * sizeof(Acc<T>);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(MELLIN_ERR_WORKSPACE, std::string(who) + ": workspace smaller than mellin_group_norm_act_workspace_bytes_*()");
-  if (!aligned_to(workspace, sizeof(Acc<T>) * 2))
-    return fail(MELLIN_ERR_WORKSPACE, std::string(who) + ": workspace must be 16-byte aligned");
-  a.chunks = chunks_for(batch, frames, channels);
+  if (!aligned_to(workspace, 16)) return fail(MELLIN_ERR_WORKSPACE, std::string(who) + ": workspace must be 16-byte aligned");
   a.part = static_cast<Acc<T> *>(workspace);
-  a.sums = a.part + (size_t)batch * a.chunks * channels * 2;
-  a.gsums = a.sums + (size_t)batch * channels * 2;
   return MELLIN_OK;
+}
+
+template <typename T>
+void prepare_twice(NormArgs<T> &a) {
+  a.chunks = chunks_for(a.batch, a.frames, a.channels);
+  a.sums = a.part + (size_t)a.batch * a.chunks * a.channels * 2;
+  a.gsums = a.sums + (size_t)a.batch * a.channels * 2;
 }
 
 template <typename T>
@@ -385,6 +817,60 @@ long long grid_for(NormArgs<T> &a, int V) {
   while (tx < 32 && tx * V < a.channels) tx *= 2;
   a.tx = tx, a.slabs = (a.channels + tx * V - 1) / (tx * V);
   return (long long)a.batch * a.chunks * a.slabs;
+}
+
+template <typename K, typename T>
+int launch(const char *who, K kernel, const NormArgs<T> &a, long long blocks, int cluster, size_t shared, cudaStream_t st) {
+  if (blocks > 0x7fffffffLL) return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many blocks");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks), cfg.blockDim = dim3(kThreads), cfg.stream = st, cfg.dynamicSmemBytes = shared;
+  if (shared > 44 * 1024) {  // with the static arrays beside it: beyond what a launch may have without asking
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 4096);
+    if (err != cudaSuccess) return fail(MELLIN_ERR_LAUNCH, std::string(who) + ": " + cudaGetErrorString(err));
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = cluster > 1 ? 1 : 0;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (err != cudaSuccess) return fail(MELLIN_ERR_LAUNCH, std::string(who) + ": " + cudaGetErrorString(err));
+  return launched(who);
+}
+
+// body(V) for the widths there are of a type
+template <typename T, typename F>
+int by_width(int V, F &&body) {
+  if (V == 1) return body(std::integral_constant<int, 1>{});
+  if (V == 2) return body(std::integral_constant<int, 2>{});
+  return body(std::integral_constant<int, 16 / (int)sizeof(T)>{});
+}
+
+template <typename T>
+void take_plan(NormArgs<T> &a, const FusedPlan &p, int V) {
+  a.team = p.team, a.col_ranks = p.col_ranks, a.row_ranks = p.row_ranks, a.kept = p.kept;
+  a.team_log2 = 0;
+  while ((1 << a.team_log2) < p.team) ++a.team_log2;
+  const int teams = kThreads / p.team;
+  a.across = (a.groups + teams - 1) / teams;
+  a.packs = a.channels / a.groups / V, a.rows = std::max(1, p.team / a.packs);
+  a.packs_magic = ((1u << 20) + a.packs - 1) / a.packs;
+}
+template <typename T, int V, int MB>
+int launch_fused(const char *who, NormArgs<T> a, const FusedPlan &p, cudaStream_t st) {
+  take_plan(a, p, V);
+  return launch(who, norm_fused_kernel<T, V, MB>, a, a.batch * p.blocks_per_utterance, p.col_ranks * p.row_ranks,
+                (size_t)p.kept * kThreads * V * sizeof(T), st);
+}
+template <typename T, int V, int MB>
+int launch_fused_backward(const char *who, NormArgs<T> &a, const FusedPlan &p, cudaStream_t st) {
+  take_plan(a, p, V);
+  a.per_block = (int)utterances_a_block(a.batch, a.frames, a.channels, p, sizeof(T));
+  const long long chunks = (a.batch + a.per_block - 1) / a.per_block;
+  a.parts = (int)(chunks * p.row_ranks);
+  const size_t shared = std::max((size_t)p.kept * kThreads * V * sizeof(T) * 2, kThreads * V * 2 * sizeof(Acc<T>));
+  const long long blocks = chunks * p.blocks_per_utterance;
+  if (a.per_block == 1) return launch(who, norm_fused_backward_kernel<T, V, MB, false>, a, blocks, p.col_ranks * p.row_ranks, shared, st);
+  return launch(who, norm_fused_backward_kernel<T, V, MB, true>, a, blocks, p.col_ranks * p.row_ranks, shared, st);
 }
 
 template <typename T>
@@ -397,22 +883,19 @@ int run_forward(NormArgs<T> a, int64_t batch, int64_t frames, int64_t channels, 
     if (frames > 0 && (a.x.p == nullptr || a.y.p == nullptr))
       return fail(MELLIN_ERR_BAD_ARGUMENT, std::string(who) + ": null pointer");
     a.eps = (Acc<T>)eps;
-    if (a.stats_out == nullptr) a.stats_out = a.gsums;
-    a.stats = a.stats_out;
     auto st = static_cast<cudaStream_t>(stream);
-    auto go = [&](auto width) -> int {
+    return by_width<T>(vector_width(a), [&](auto width) -> int {
       constexpr int V = decltype(width)::value;
+      const FusedPlan p = plan_fused(batch, frames, groups, channels / groups, V, 1, sizeof(T));
+      if (p.use) return launch_fused<T, V, sizeof(T) == 2 ? 3 : 2>(who, a, p, st);
+      prepare_twice(a);
+      if (a.stats_out == nullptr) a.stats_out = a.gsums;
+      a.stats = a.stats_out;
       const long long blocks = grid_for(a, V);
-      if (blocks > 0x7fffffffLL) return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many blocks");
-      norm_moments_kernel<T, V><<<(unsigned)blocks, kThreads, 0, st>>>(a);
-      if ((rc = launched(who)) != MELLIN_OK) return rc;
-      norm_stats_kernel<T><<<(unsigned)(batch * groups), kThreads, 0, st>>>(a);
-      if ((rc = launched(who)) != MELLIN_OK || frames == 0) return rc;
-      norm_apply_kernel<T, V><<<(unsigned)blocks, kThreads, 0, st>>>(a);
-      return launched(who);
-    };
-    constexpr int V = 16 / sizeof(T);
-    return vector_width(a) == V ? go(std::integral_constant<int, V>{}) : go(std::integral_constant<int, 1>{});
+      if ((rc = launch(who, norm_moments_kernel<T, V>, a, blocks, 1, 0, st)) != MELLIN_OK) return rc;
+      if ((rc = launch(who, norm_stats_kernel<T>, a, batch * groups, 1, 0, st)) != MELLIN_OK) return rc;
+      return launch(who, norm_apply_kernel<T, V>, a, blocks, 1, 0, st);
+    });
   });
 }
 
@@ -424,27 +907,34 @@ int run_backward(NormArgs<T> a, int64_t batch, int64_t frames, int64_t channels,
     int rc = prepare(who, a, batch, frames, channels, groups, act, workspace, workspace_bytes);
     if (rc != MELLIN_OK || channels == 0) return rc;
     auto st = static_cast<cudaStream_t>(stream);
-    const unsigned param_blocks = (unsigned)((channels + kThreads - 1) / kThreads);
+    const Acc<T> *sums = nullptr;
+    int parts = 0;
     if (batch > 0) {
       if (a.stats == nullptr || (frames > 0 && (a.x.p == nullptr || a.grad_y.p == nullptr || a.grad_x.p == nullptr)))
         return fail(MELLIN_ERR_BAD_ARGUMENT, std::string(who) + ": null pointer");
-      auto go = [&](auto width) -> int {
+      rc = by_width<T>(vector_width(a), [&](auto width) -> int {
         constexpr int V = decltype(width)::value;
+        const FusedPlan p = plan_fused(batch, frames, groups, channels / groups, V, 2, sizeof(T));
+        if (p.use) {
+          rc = launch_fused_backward<T, V, 2>(who, a, p, st);
+          parts = a.parts, sums = a.part;
+          return rc;
+        }
+        prepare_twice(a);
+        parts = (int)batch, sums = a.sums;
         const long long blocks = grid_for(a, V);
-        if (blocks > 0x7fffffffLL) return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many blocks");
-        norm_sums_kernel<T, V><<<(unsigned)blocks, kThreads, 0, st>>>(a);
-        if ((rc = launched(who)) != MELLIN_OK) return rc;
-        norm_group_sums_kernel<T><<<(unsigned)(batch * groups), kThreads, 0, st>>>(a);
-        if ((rc = launched(who)) != MELLIN_OK || frames == 0) return rc;
-        norm_grad_input_kernel<T, V><<<(unsigned)blocks, kThreads, 0, st>>>(a);
-        return launched(who);
-      };
-      constexpr int V = 16 / sizeof(T);
-      rc = vector_width(a) == V ? go(std::integral_constant<int, V>{}) : go(std::integral_constant<int, 1>{});
-      if (rc != MELLIN_OK) return rc;
+        if ((rc = launch(who, norm_sums_kernel<T, V>, a, blocks, 1, 0, st)) != MELLIN_OK) return rc;
+        if ((rc = launch(who, norm_group_sums_kernel<T>, a, batch * groups, 1, 0, st)) != MELLIN_OK) return rc;
+        rc = launch(who, norm_grad_input_kernel<T, V>, a, blocks, 1, 0, st);
+        a.parts = 0;  // the sums are still to be added, whatever their number
+        return rc;
+      });
+      if (rc != MELLIN_OK || a.parts == 1) return rc;
     }
     if (a.grad_weight == nullptr && a.grad_bias == nullptr) return MELLIN_OK;
-    norm_grad_params_kernel<T><<<param_blocks, kThreads, 0, st>>>(a);
+    const cudaError_t err = launch_after_predecessor(norm_grad_params_kernel<T>, dim3((unsigned)((channels + 31) / 32)),
+                                                     dim3(kThreads), 0, st, a, sums, parts);
+    if (err != cudaSuccess) return fail(MELLIN_ERR_LAUNCH, std::string(who) + ": " + cudaGetErrorString(err));
     return launched(who);
   });
 }
@@ -455,8 +945,9 @@ int run_backward(NormArgs<T> a, int64_t batch, int64_t frames, int64_t channels,
 using namespace mellin;
 
 #define NORM_ENTRIES(SUFFIX, T, P, S)                                                                                  \
-  size_t mellin_group_norm_act_workspace_bytes_##SUFFIX(int64_t batch, int64_t frames, int64_t channels) {             \
-    return workspace_elements(batch, frames, channels) * sizeof(S);                                                    \
+  size_t mellin_group_norm_act_workspace_bytes_##SUFFIX(int64_t batch, int64_t frames, int64_t channels,               \
+                                                        int64_t groups) {                                              \
+    return workspace_elements(batch, frames, channels, groups, sizeof(T)) * sizeof(S);                                 \
   }                                                                                                                    \
   int mellin_group_norm_act_##SUFFIX(const P *x, int64_t x_sn, int64_t x_st, const S *weight, const S *bias,           \
                                      const int *lens, int64_t batch, int64_t frames, int64_t channels, int64_t groups, \

@@ -15,7 +15,6 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <climits>
 
 #include "sequence_common.cuh"
 
@@ -135,22 +134,6 @@ __device__ __forceinline__ void load_acc(A (&to)[V], const A *from) {
   }
 }
 
-// Which utterance a block takes that is `turn`th in launch order: the longest first, so that the last blocks to start
-// are short ones (32 utterances of 200 to 800 frames, 1024 channels, bfloat16: forward 36 -> 32 us, backward 55 -> 47).
-// Every warp sorts for itself, lane i counting what goes before utterance i; batches above 32, whose blocks are many
-// enough to even out, are taken as they come.
-__device__ __forceinline__ int utterance_of(const int *lens, int batch, int turn) {
-  if (lens == nullptr || batch > 32 || batch == 1) return turn;
-  const int lane = threadIdx.x & 31, mine = lane < batch ? lens[lane] : INT_MIN;
-  int place = 0;
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const int other = __shfl_sync(0xffffffffu, mine, j);
-    place += other > mine || (other == mine && j < lane);
-  }
-  return __ffs(__ballot_sync(0xffffffffu, place == turn)) - 1;
-}
-
 template <typename A, int CT, int W>
 struct alignas(16) ScanShared {
   A a[2][W][CT], b[2][W][CT], carry[2][CT];
@@ -162,10 +145,11 @@ __global__ void __launch_bounds__(32 * W, MB) recurrence_scan_kernel(const Recur
   __shared__ ScanShared<A, CT, W> sh;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, cl = lane % CL, tl = lane / CL, at = cl * V;
   const int unit = (int)blockIdx.x;
-  const long long n = utterance_of(a.lens, a.batch, unit / a.tiles);
+  const Utterance whose = utterance_of(a.lens, a.batch, a.frames, unit / a.tiles);
+  const long long n = whose.n;
   const int c = unit % a.tiles * CT + at;
   const bool on = c < a.channels;
-  const int len = live_frames(a.lens, n, a.frames), steps = (len + SPAN - 1) / SPAN;
+  const int len = whose.len, steps = (len + SPAN - 1) / SPAN;
   const int slots = (a.frames + kStateStride - 1) / kStateStride;
   const int mine = w * kStateStride + tl * S;  // this thread's first frame of step 0
   const T *x = a.x.p + n * a.x.sn + c, *gate = a.gate.p + n * a.gate.sn + c;
@@ -292,10 +276,11 @@ __global__ void __launch_bounds__(32 * W, MB) recurrence_scan_backward_kernel(co
   __shared__ ScanShared<A, CT, W> sh;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, cl = lane % CL, tl = lane / CL, at = cl * V;
   const int unit = (int)blockIdx.x;
-  const long long n = utterance_of(a.lens, a.batch, unit / a.tiles);
+  const Utterance whose = utterance_of(a.lens, a.batch, a.frames, unit / a.tiles);
+  const long long n = whose.n;
   const int c = unit % a.tiles * CT + at;
   const bool on = c < a.channels;
-  const int len = live_frames(a.lens, n, a.frames), steps = (len + SPAN - 1) / SPAN;
+  const int len = whose.len, steps = (len + SPAN - 1) / SPAN;
   const int slots = (a.frames + kStateStride - 1) / kStateStride;
   const int mine = w * kStateStride + tl * S;
   const T *x = a.x.p + n * a.x.sn + c, *gate = a.gate.p + n * a.gate.sn + c;

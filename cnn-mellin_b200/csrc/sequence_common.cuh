@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <climits>
 #include <cstdint>
 #include <exception>
 #include <string>
@@ -47,6 +48,34 @@ __device__ __forceinline__ __nv_bfloat16 from_acc<__nv_bfloat16>(float v) {
 }
 
 inline bool aligned_to(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
+
+// frames of utterance n that exist: lens[n] held inside [0, frames]; all of them without lens
+__device__ __forceinline__ int live_frames(const int *lens, long long n, int frames) {
+  if (lens == nullptr) return frames;
+  const int v = lens[n];
+  return v < 0 ? 0 : (v > frames ? frames : v);
+}
+
+// Which utterance a block takes that is `turn`th in launch order, and its frames: the longest first, so that the last
+// blocks to start are short ones (recurrence, 32 utterances of 200 to 800 frames, 1024 channels, bfloat16: forward
+// 36 -> 32 us, backward 55 -> 47).  Every warp sorts for itself, lane i counting what goes before utterance i (one warp
+// and a block barrier: 5 % slower); batches above 32, whose blocks are many enough to even out, are taken as they come.
+struct Utterance {
+  int n, len;
+};
+__device__ __forceinline__ Utterance utterance_of(const int *lens, int batch, int frames, int turn) {
+  if (lens == nullptr) return {turn, frames};
+  if (batch > 32 || batch == 1) return {turn, live_frames(lens, turn, frames)};
+  const int lane = threadIdx.x & 31, mine = lane < batch ? lens[lane] : INT_MIN;
+  int place = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const int other = __shfl_sync(0xffffffffu, mine, j);
+    place += other > mine || (other == mine && j < lane);
+  }
+  const int n = __ffs(__ballot_sync(0xffffffffu, place == turn)) - 1, len = __shfl_sync(0xffffffffu, mine, n);
+  return {n, len < 0 ? 0 : (len > frames ? frames : len)};
+}
 
 // V consecutive elements as the 32-bit words they lie in, moved by accesses of up to 16 bytes (one address, a multiple of
 // the access); elements are taken out of the words only where they are used, so that loads can stay in flight.
@@ -110,6 +139,39 @@ __device__ __forceinline__ float element(const Raw<__half, V> &r, int v) {
   return __half2float(__ushort_as_half((unsigned short)(v & 1 ? r.w[v / 2] >> 16 : r.w[v / 2])));
 }
 
+// V elements from global to shared memory without a register between; complete after copies_done() in the same thread.
+// Two-byte packs, which the asynchronous copy does not know, are loaded and stored.
+template <typename T, int V>
+__device__ __forceinline__ void copy_async(T *to, const T *from) {
+  constexpr int BYTES = Raw<T, V>::kBytes;
+  if constexpr (BYTES == 2) {
+    store_raw<T, V>(to, load_raw<T, V>(from));
+  } else {
+    const unsigned dst = (unsigned)__cvta_generic_to_shared(to);
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(from), "n"(BYTES) : "memory");
+  }
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> load_shared(const T *p) {
+  Raw<T, V> r;
+  constexpr int BYTES = Raw<T, V>::kBytes;
+  static_assert(BYTES <= 16, "one access");
+  if constexpr (BYTES == 2) {
+    r.w[0] = *reinterpret_cast<const unsigned short *>(p);
+  } else if constexpr (BYTES == 4) {
+    r.w[0] = *reinterpret_cast<const unsigned *>(p);
+  } else if constexpr (BYTES == 8) {
+    const uint2 q = *reinterpret_cast<const uint2 *>(p);
+    r.w[0] = q.x, r.w[1] = q.y;
+  } else {
+    const uint4 q = *reinterpret_cast<const uint4 *>(p);
+    r.w[0] = q.x, r.w[1] = q.y, r.w[2] = q.z, r.w[3] = q.w;
+  }
+  return r;
+}
+
 // V values rounded to T
 template <typename T, int V>
 __device__ __forceinline__ Raw<T, V> rounded(const Acc<T> (&a)[V]) {
@@ -166,13 +228,6 @@ struct Frames {
   long long sn = 0, st = 0;
 };
 
-// frames of utterance n that exist: lens[n] held inside [0, frames]; all of them without lens
-__device__ __forceinline__ int live_frames(const int *lens, long long n, int frames) {
-  if (lens == nullptr) return frames;
-  const int v = lens[n];
-  return v < 0 ? 0 : (v > frames ? frames : v);
-}
-
 // 2^v and 1 / v by the special function unit alone, without the scaling around it that results below 2^-126 need
 __device__ __forceinline__ float exp2_unit(float v) {
   float r;
@@ -184,6 +239,15 @@ __device__ __forceinline__ float reciprocal_unit(float v) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+
+__device__ __forceinline__ double reciprocal_unit(double v) { return 1.0 / v; }
+// the larger one; NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ double max_nan(double a, double b) { return a > b ? a : (a <= b ? b : a + b); }
 
 // sigmoid(g) and 1 - sigmoid(g), each to a few units in its own last place: the complement is e sigmoid(g) with
 // e = exp(-g), not a difference.  e is held at 2^126, so that the quotient stays a normal number (the least sigmoid is

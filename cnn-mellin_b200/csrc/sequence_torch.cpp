@@ -261,8 +261,8 @@ std::tuple<Tensor, Tensor> norm_forward(const Tensor &input, int64_t groups, con
     using A = decltype(api);
     using P = typename A::P;
     using S = typename A::S;
-    const size_t bytes = A::norm_workspace(n, t, channels);
-    const Tensor ws = at::empty({static_cast<int64_t>(bytes)}, input.options().dtype(at::kByte));
+    const size_t bytes = A::norm_workspace(n, t, channels, groups);
+    const Tensor ws = bytes > 0 ? at::empty({static_cast<int64_t>(bytes)}, input.options().dtype(at::kByte)) : Tensor();
     return A::norm(ptr<P>(x), x.stride(0), x.stride(1), ptr<S>(w), ptr<S>(b), lens_ptr(lens), n, t, channels, groups, eps,
                    static_cast<int>(act), ptr<P>(y), y.stride(0), y.stride(1), ptr<S>(stats), ptr<void>(ws), bytes,
                    current_stream(input));
@@ -302,8 +302,8 @@ class GroupNormActFunction : public torch::autograd::Function<GroupNormActFuncti
         using A = decltype(api);
         using P = typename A::P;
         using S = typename A::S;
-        const size_t bytes = A::norm_workspace(n, t, channels);
-        const Tensor ws = at::empty({static_cast<int64_t>(bytes)}, input.options().dtype(at::kByte));
+        const size_t bytes = A::norm_workspace(n, t, channels, ctx->saved_data["groups"].toInt());
+        const Tensor ws = bytes > 0 ? at::empty({static_cast<int64_t>(bytes)}, input.options().dtype(at::kByte)) : Tensor();
         return A::norm_backward(ptr<P>(x), x.stride(0), x.stride(1), ptr<S>(w), ptr<S>(b), ptr<S>(stats), lens_ptr(lens), n,
                                 t, channels, ctx->saved_data["groups"].toInt(),
                                 static_cast<int>(ctx->saved_data["act"].toInt()), ptr<P>(gy), gy.stride(0), gy.stride(1),

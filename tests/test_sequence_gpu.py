@@ -231,6 +231,14 @@ NORMS = [
     (2, 100, 72, 2, None, "silu", True, "channels apart"),
     (1, 1500, 40, 5, [1499], "silu", True, "dense"),
     (1, 3001, 512, 2, None, "gelu", True, "wide"),
+    (2, 500, 256, 1, [500, 490], "silu", True, "dense"),
+    (2, 900, 256, 1, None, "relu", True, "dense"),
+    (2, 100, 256, 1, [100, 3], "none", True, "odd"),
+    (3, 20, 1200, 1, None, "silu", True, "dense"),
+    (3, 20, 1200, 1, [20, 0, 19], "gelu", True, "odd"),
+    (2, 5, 4100, 1, None, "silu", True, "odd"),
+    (2500, 1, 32, 4, None, "relu", True, "dense"),
+    (1100, 2, 10, 5, [i % 3 for i in range(1100)], "silu", True, "time-major"),
 ]
 
 
