@@ -11,8 +11,11 @@ Adam with learning rate 1e-4, FP32 throughout.
 
 Only the convolutional layers are this package's kernels; the per-frame
 matrix products, the loss and the optimizer are stock PyTorch, as they are in
-the reference.  Data is synthetic: N(0, 1) features of ragged length, random
-label sequences.
+the reference.  With ``sequence_layers`` > 0, residual sequence blocks
+(``sequence.SequenceBlock``: norm, two-way gated recurrence, dropout) stand
+between the hidden layers and the output, where the reference's model has its
+recurrent layers (``models.py:435-445``).  Data is synthetic: N(0, 1) features
+of ragged length, random label sequences.
 """
 from typing import List, Optional, Sequence, Tuple
 
@@ -20,6 +23,7 @@ import torch
 import torch.nn.functional as F
 
 import mconv
+import sequence
 
 BINS = 41
 CLASSES = 62  # 61 phones + blank (the last index, as running.py:240)
@@ -46,26 +50,31 @@ class _PackFrames(torch.autograd.Function):
 
 
 class _UnpackFrames(torch.autograd.Function):
-    """(C, sum of lengths) -> (T, N, C) padded with zeros: the layout the CTC loss reads."""
+    """(C, sum of lengths) -> (T, N, C) padded with zeros: the layout the CTC loss reads; or, ``batch_first``, (N, T, C),
+    the layout of the sequence operators."""
 
     @staticmethod
-    def forward(ctx, packed, lengths, t):
-        ctx.lengths = lengths
-        out = packed.new_zeros((t, len(lengths), packed.shape[0]))
+    def forward(ctx, packed, lengths, t, batch_first=False):
+        ctx.lengths, ctx.batch_first = lengths, batch_first
+        n_all, c = len(lengths), packed.shape[0]
+        out = packed.new_zeros((n_all, t, c) if batch_first else (t, n_all, c))
+        frames = out if batch_first else out.transpose(0, 1)
         o = 0
         for i, n in enumerate(lengths):
-            out[:n, i] = packed[:, o:o + n].t()
+            frames[i, :n] = packed[:, o:o + n].t()
             o += n
         return out
 
     @staticmethod
     def backward(ctx, grad):
-        return torch.cat([grad[:n, i].t() for i, n in enumerate(ctx.lengths)], dim=1), None, None
+        frames = grad if ctx.batch_first else grad.transpose(0, 1)
+        return torch.cat([frames[i, :n].t() for i, n in enumerate(ctx.lengths)], dim=1), None, None, None
 
 
 class MellinCTCNet(torch.nn.Module):
     def __init__(self, channels: Sequence[int] = CHANNELS, kernel: Tuple[int, int] = KERNEL, bins: int = BINS,
-                 hidden: int = 1024, classes: int = CLASSES, dropout: float = 0.05, fused_dropout: bool = True):
+                 hidden: int = 1024, classes: int = CLASSES, dropout: float = 0.05, fused_dropout: bool = True,
+                 sequence_layers: int = 0, sequence_groups: int = 32):
         super().__init__()
         valid = mconv.mcorr_valid_size(kernel[0], bins)
         same = (bins - valid, 1)  # same-size output on both axes (time padding 1)
@@ -79,6 +88,8 @@ class MellinCTCNet(torch.nn.Module):
         self.fused_dropout = fused_dropout  # False: torch's dropout as a separate pass (for comparison)
         self.fc1 = torch.nn.Linear(channels[-1] * bins, hidden)
         self.fc2 = torch.nn.Linear(hidden, hidden)
+        self.blocks = torch.nn.ModuleList(
+            sequence.SequenceBlock(hidden, num_groups=sequence_groups, dropout=dropout) for _ in range(sequence_layers))
         self.out = torch.nn.Linear(hidden, classes)
 
     def forward(self, x: torch.Tensor, lens: torch.Tensor) -> torch.Tensor:
@@ -99,6 +110,11 @@ class MellinCTCNet(torch.nn.Module):
         h = _PackFrames.apply(x.reshape(n, c * b, t), lengths)                        # (features, valid frames)
         h = F.relu(torch.addmm(self.fc1.bias[:, None], self.fc1.weight, h))
         h = F.relu(torch.addmm(self.fc2.bias[:, None], self.fc2.weight, h))
+        if len(self.blocks):
+            seq = _UnpackFrames.apply(h, lengths, t, True)                            # (N, T, hidden), padded
+            for block in self.blocks:
+                seq, _ = block(seq, lens)
+            return F.log_softmax(self.out(seq), dim=2).transpose(0, 1)                # (T, N, classes)
         logits = torch.addmm(self.out.bias[:, None], self.out.weight, h)              # (classes, valid frames)
         # back to the padded (T, N, classes) layout the loss expects; frames past an utterance's end are never read
         return _UnpackFrames.apply(F.log_softmax(logits, dim=0), lengths, t)

@@ -188,7 +188,8 @@ class SequenceBlock(torch.nn.Module):
 
     ``forward(x, lens=None, state=None)`` returns ``(output, state)``.  ``streaming``: one way and the norm frame by frame,
     so that feeding a stream in pieces with the state passed on gives what one call over all of it gives; otherwise the
-    recurrence runs both ways and the norm's statistics are an utterance's."""
+    recurrence runs both ways and the norm's statistics are an utterance's.  Frames behind an utterance's end come out
+    as they went in plus the output layer's bias: finite where ``x`` is, and never read by the next block."""
 
     def __init__(self, channels: int, hidden: Optional[int] = None, num_groups: int = 32, activation: str = "silu",
                  dropout: float = 0.05, streaming: bool = False):
