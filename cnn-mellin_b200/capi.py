@@ -82,7 +82,7 @@ def lib():
         _lib.mellin_gated_recurrence_state_count.restype = _I64
         for sfx in ("_f32", "_f64", "_f16", "_bf16"):
             fn = getattr(_lib, "mellin_group_norm_act_workspace_bytes" + sfx)
-            fn.restype, fn.argtypes = ctypes.c_size_t, [_I64] * 4
+            fn.restype, fn.argtypes = ctypes.c_size_t, [_I64] * 4 + [_INT]
     return _lib
 
 

@@ -768,12 +768,12 @@ int64_t utterances_a_block(int64_t batch, int64_t frames, int64_t channels, cons
   return std::max<int64_t>(1, batch * p.blocks_per_utterance / (148 * 6));
 }
 
-// workspace in elements of the accumulation type.  The fused kernels need the sets of parameter sums only; the others (batch, chunks, channels, 2), (batch, channels, 2) and (batch, groups, 2).
-size_t workspace_elements(int64_t batch, int64_t frames, int64_t channels, int64_t groups, size_t element) {
+// workspace in elements of the accumulation type.  The fused kernels need the sets of parameter sums, backward; the others (batch, chunks, channels, 2), (batch, channels, 2) and (batch, groups, 2).
+size_t workspace_elements(int64_t batch, int64_t frames, int64_t channels, int64_t groups, size_t element, bool backward) {
   if (batch <= 0 || frames < 0 || channels <= 0 || groups <= 0 || channels % groups != 0) return 0;
   size_t need = 0;
   for (int V : {1, 2, 4, 8}) {
-    if (channels / groups % V != 0) continue;
+    if (!backward || channels / groups % V != 0) continue;
     const FusedPlan p = plan_fused(batch, frames, groups, channels / groups, V, 2, element);
     if (!p.use) continue;
     const int64_t each = utterances_a_block(batch, frames, channels, p, element);
@@ -786,7 +786,7 @@ size_t workspace_elements(int64_t batch, int64_t frames, int64_t channels, int64
 
 template <typename T>
 int prepare(const char *who, NormArgs<T> &a, int64_t batch, int64_t frames, int64_t channels, int64_t groups, int act,
-            void *workspace, size_t workspace_bytes) {
+            bool backward, void *workspace, size_t workspace_bytes) {
   const int rc = check_extents(who, batch, frames, channels);
   if (rc != MELLIN_OK) return rc;
   if (groups <= 0 || channels % groups != 0)
@@ -796,7 +796,7 @@ int prepare(const char *who, NormArgs<T> &a, int64_t batch, int64_t frames, int6
     return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many utterances times channels");
   a.batch = (int)batch, a.frames = (int)frames, a.channels = (int)channels, a.groups = (int)groups, a.act = act;
   if (batch == 0 || channels == 0) return MELLIN_OK;
-  const size_t need = workspace_elements(batch, frames, channels, groups, sizeof(T)) * sizeof(Acc<T>);
+  const size_t need = workspace_elements(batch, frames, channels, groups, sizeof(T), backward) * sizeof(Acc<T>);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(MELLIN_ERR_WORKSPACE, std::string(who) + ": workspace smaller than mellin_group_norm_act_workspace_bytes_*()");
   if (!aligned_to(workspace, 16)) return fail(MELLIN_ERR_WORKSPACE, std::string(who) + ": workspace must be 16-byte aligned");
@@ -878,7 +878,7 @@ int run_forward(NormArgs<T> a, int64_t batch, int64_t frames, int64_t channels, 
                 void *workspace, size_t workspace_bytes, void *stream) {
   const char *who = "group_norm_act";
   return guarded(who, [&]() -> int {
-    int rc = prepare(who, a, batch, frames, channels, groups, act, workspace, workspace_bytes);
+    int rc = prepare(who, a, batch, frames, channels, groups, act, false, workspace, workspace_bytes);
     if (rc != MELLIN_OK || batch == 0 || channels == 0) return rc;
     if (frames > 0 && (a.x.p == nullptr || a.y.p == nullptr))
       return fail(MELLIN_ERR_BAD_ARGUMENT, std::string(who) + ": null pointer");
@@ -904,7 +904,7 @@ int run_backward(NormArgs<T> a, int64_t batch, int64_t frames, int64_t channels,
                  void *workspace, size_t workspace_bytes, void *stream) {
   const char *who = "backward of group_norm_act";
   return guarded(who, [&]() -> int {
-    int rc = prepare(who, a, batch, frames, channels, groups, act, workspace, workspace_bytes);
+    int rc = prepare(who, a, batch, frames, channels, groups, act, true, workspace, workspace_bytes);
     if (rc != MELLIN_OK || channels == 0) return rc;
     auto st = static_cast<cudaStream_t>(stream);
     const Acc<T> *sums = nullptr;
@@ -946,8 +946,8 @@ using namespace mellin;
 
 #define NORM_ENTRIES(SUFFIX, T, P, S)                                                                                  \
   size_t mellin_group_norm_act_workspace_bytes_##SUFFIX(int64_t batch, int64_t frames, int64_t channels,               \
-                                                        int64_t groups) {                                              \
-    return workspace_elements(batch, frames, channels, groups, sizeof(T)) * sizeof(S);                                 \
+                                                        int64_t groups, int backward) {                                \
+    return workspace_elements(batch, frames, channels, groups, sizeof(T), backward != 0) * sizeof(S);                  \
   }                                                                                                                    \
   int mellin_group_norm_act_##SUFFIX(const P *x, int64_t x_sn, int64_t x_st, const S *weight, const S *bias,           \
                                      const int *lens, int64_t batch, int64_t frames, int64_t channels, int64_t groups, \

@@ -61,6 +61,11 @@ void *current_stream(const Tensor &t) {
 }
 
 at::ScalarType state_type(const Tensor &t) { return t.scalar_type() == at::kDouble ? at::kDouble : at::kFloat; }
+// a state or parameter as the C ABI takes it
+Tensor as_state(const Tensor &input, const OptTensor &p) {
+  if (!p) return Tensor();
+  return p->scalar_type() == state_type(input) && p->is_contiguous() ? *p : p->to(state_type(input)).contiguous();
+}
 
 // ---- checks ---------------------------------------------------------------------------------------------------------
 
@@ -103,7 +108,7 @@ Tensor empty_frames(const Tensor &like, int64_t channels) {
 }
 
 const int *lens_ptr(const OptTensor &lens) { return lens && lens->numel() > 0 ? lens->data_ptr<int>() : nullptr; }
-OptTensor dense(const OptTensor &lens) { return lens ? OptTensor(lens->contiguous()) : lens; }
+OptTensor dense(const OptTensor &lens) { return lens && !lens->is_contiguous() ? OptTensor(lens->contiguous()) : lens; }
 
 // gradients that a second differentiation would silently miss: refuse it when it comes to that
 tensor_list once_differentiable(const char *what, tensor_list grads) {
@@ -124,15 +129,17 @@ bool wants_grad(const OptTensor &t) { return t && t->requires_grad(); }
 
 // ---- gated recurrence -----------------------------------------------------------------------------------------------
 
-struct Mix {
-  Tensor x, gate;
+// What the C ABI takes of a (batch, frames, channels) tensor, or of its channels from `first` on: no tensor is made for it
+struct View {
+  void *p = nullptr;
+  int64_t sn = 0, st = 0;
+  View() = default;
+  explicit View(const Tensor &t, int64_t first = 0) {
+    if (!t.defined() || t.numel() == 0) return;
+    p = static_cast<char *>(t.data_ptr()) + first * t.element_size();
+    sn = t.stride(0), st = t.stride(1);
+  }
 };
-Mix split(const Tensor &input, const OptTensor &gate) {
-  if (gate) return {frames_view(input), frames_view(*gate)};
-  const int64_t channels = input.size(2) / 2;
-  const Tensor t = frames_view(input);
-  return {t.narrow(2, 0, channels), t.narrow(2, channels, channels)};
-}
 
 // (output, final state, states kept for backward)
 std::tuple<Tensor, Tensor, Tensor> recurrence_forward(const Tensor &input, const OptTensor &gate, const OptTensor &initial,
@@ -150,19 +157,19 @@ std::tuple<Tensor, Tensor, Tensor> recurrence_forward(const Tensor &input, const
   if (initial) check_like(c, *initial, "initial", input, {n, channels});
   check_lens(c, lens_in, input);
   c10::cuda::CUDAGuard guard(input.device());
-  const Mix m = split(input, gate);
+  const Tensor in = frames_view(input), gate_in = gate ? frames_view(*gate) : in;
+  const View x(in), g(gate_in, gate ? 0 : channels);
   const OptTensor lens = dense(lens_in);
   const auto state_options = input.options().dtype(state_type(input));
-  const Tensor h0 = initial ? initial->to(state_type(input)).contiguous() : Tensor();
+  const Tensor h0 = as_state(input, initial);
   Tensor y = empty_frames(input, channels), final = at::empty({n, channels}, state_options), states;
   if (keep_states) states = at::empty({mellin_gated_recurrence_state_count(n, t, channels)}, state_options);
   check_status(by_type(input.scalar_type(), [&](auto api) {
     using A = decltype(api);
     using P = typename A::P;
     using S = typename A::S;
-    return A::recurrence(ptr<P>(m.x), m.x.stride(0), m.x.stride(1), ptr<P>(m.gate), m.gate.stride(0), m.gate.stride(1),
-                         ptr<S>(h0), lens_ptr(lens), reverse ? 1 : 0, n, t, channels, ptr<P>(y), y.stride(0), y.stride(1),
-                         ptr<S>(final), ptr<S>(states), current_stream(input));
+    return A::recurrence(static_cast<P *>(x.p), x.sn, x.st, static_cast<P *>(g.p), g.sn, g.st, ptr<S>(h0), lens_ptr(lens),
+                         reverse ? 1 : 0, n, t, channels, ptr<P>(y), y.stride(0), y.stride(1), ptr<S>(final), ptr<S>(states), current_stream(input));
   }), c);
   return {y, final, states};
 }
@@ -192,18 +199,15 @@ class GatedRecurrenceFunction : public torch::autograd::Function<GatedRecurrence
     const OptTensor gate = saved[1].defined() ? OptTensor(saved[1]) : OptTensor();
     const OptTensor lens = dense(saved[3].defined() ? OptTensor(saved[3]) : OptTensor());
     const int64_t initial_type = ctx->saved_data["initial"].toInt();
-    Tensor gx, gg, gi, whole;
+    Tensor gx, gg, gi;  // without a gate tensor, gx holds both gradients
     {
       at::AutoDispatchBelowADInplaceOrView below;
       c10::cuda::CUDAGuard guard(input.device());
-      const Mix m = split(input, gate);
-      const int64_t n = m.x.size(0), t = m.x.size(1), channels = m.x.size(2);
-      if (gate) {
-        gx = empty_frames(input, channels), gg = empty_frames(*gate, channels);
-      } else {
-        whole = empty_frames(input, 2 * channels);
-        gx = whole.narrow(2, 0, channels), gg = whole.narrow(2, channels, channels);
-      }
+      const Tensor in = frames_view(input), gate_in = gate ? frames_view(*gate) : in;
+      const int64_t n = in.size(0), t = in.size(1), channels = gate ? in.size(2) : in.size(2) / 2;
+      gx = empty_frames(input, in.size(2));
+      if (gate) gg = empty_frames(*gate, channels);
+      const View x(in), g(gate_in, gate ? 0 : channels), ox(gx), og(gate ? gg : gx, gate ? 0 : channels);
       const Tensor gy = grads[0].defined() ? frames_view(grads[0]) : Tensor();
       const Tensor gf = grads[1].defined() ? grads[1].contiguous() : Tensor();
       if (initial_type >= 0) gi = at::empty({n, channels}, input.options().dtype(state_type(input)));
@@ -212,15 +216,15 @@ class GatedRecurrenceFunction : public torch::autograd::Function<GatedRecurrence
         using P = typename A::P;
         using S = typename A::S;
         return A::recurrence_backward(
-            ptr<P>(m.x), m.x.stride(0), m.x.stride(1), ptr<P>(m.gate), m.gate.stride(0), m.gate.stride(1), ptr<S>(states),
-            lens_ptr(lens), ctx->saved_data["reverse"].toBool() ? 1 : 0, n, t, channels, ptr<P>(gy),
-            gy.defined() ? gy.stride(0) : 0, gy.defined() ? gy.stride(1) : 0, ptr<S>(gf), ptr<P>(gx), gx.stride(0),
-            gx.stride(1), ptr<P>(gg), gg.stride(0), gg.stride(1), ptr<S>(gi), current_stream(input));
+            static_cast<P *>(x.p), x.sn, x.st, static_cast<P *>(g.p), g.sn, g.st, ptr<S>(states), lens_ptr(lens),
+            ctx->saved_data["reverse"].toBool() ? 1 : 0, n, t, channels, ptr<P>(gy), gy.defined() ? gy.stride(0) : 0,
+            gy.defined() ? gy.stride(1) : 0, ptr<S>(gf), static_cast<P *>(ox.p), ox.sn, ox.st, static_cast<P *>(og.p), og.sn,
+            og.st, ptr<S>(gi), current_stream(input));
       }), c);
-      if (gi.defined()) gi = gi.to(static_cast<at::ScalarType>(initial_type));
+      if (gi.defined() && static_cast<int64_t>(gi.scalar_type()) != initial_type)
+        gi = gi.to(static_cast<at::ScalarType>(initial_type));
     }
-    return once_differentiable("gated_recurrence",
-                               {gate ? gx : whole, gate ? gg : Tensor(), gi, Tensor(), Tensor()});
+    return once_differentiable("gated_recurrence", {gx, gg, gi, Tensor(), Tensor()});
   }
 };
 
@@ -236,10 +240,6 @@ std::tuple<Tensor, Tensor> gated_recurrence_autograd(const Tensor &input, const 
 
 // ---- group norm with an activation ----------------------------------------------------------------------------------
 
-Tensor parameter(const Tensor &input, const OptTensor &p) {
-  return p ? p->to(state_type(input)).contiguous() : Tensor();
-}
-
 // (output, statistics) of a (batch, frames, channels) tensor
 std::tuple<Tensor, Tensor> norm_forward(const Tensor &input, int64_t groups, const OptTensor &weight, const OptTensor &bias,
                                         const OptTensor &lens_in, double eps, int64_t act, bool keep_stats) {
@@ -253,7 +253,7 @@ std::tuple<Tensor, Tensor> norm_forward(const Tensor &input, int64_t groups, con
   if (bias) check_like(c, *bias, "bias", input, {channels});
   check_lens(c, lens_in, input);
   c10::cuda::CUDAGuard guard(input.device());
-  const Tensor x = frames_view(input), w = parameter(input, weight), b = parameter(input, bias);
+  const Tensor x = frames_view(input), w = as_state(input, weight), b = as_state(input, bias);
   const OptTensor lens = dense(lens_in);
   Tensor y = empty_frames(input, channels), stats;
   if (keep_stats) stats = at::empty({n, groups, 2}, input.options().dtype(state_type(input)));
@@ -261,7 +261,7 @@ std::tuple<Tensor, Tensor> norm_forward(const Tensor &input, int64_t groups, con
     using A = decltype(api);
     using P = typename A::P;
     using S = typename A::S;
-    const size_t bytes = A::norm_workspace(n, t, channels, groups);
+    const size_t bytes = A::norm_workspace(n, t, channels, groups, 0);
     const Tensor ws = bytes > 0 ? at::empty({static_cast<int64_t>(bytes)}, input.options().dtype(at::kByte)) : Tensor();
     return A::norm(ptr<P>(x), x.stride(0), x.stride(1), ptr<S>(w), ptr<S>(b), lens_ptr(lens), n, t, channels, groups, eps,
                    static_cast<int>(act), ptr<P>(y), y.stride(0), y.stride(1), ptr<S>(stats), ptr<void>(ws), bytes,
@@ -293,7 +293,7 @@ class GroupNormActFunction : public torch::autograd::Function<GroupNormActFuncti
       c10::cuda::CUDAGuard guard(input.device());
       const int64_t n = input.size(0), t = input.size(1), channels = input.size(2);
       const Tensor x = frames_view(input), gy = frames_view(grads[0]);
-      const Tensor w = parameter(input, weight), b = parameter(input, bias);
+      const Tensor w = as_state(input, weight), b = as_state(input, bias);
       gx = empty_frames(input, channels);
       const auto options = input.options().dtype(state_type(input));
       if (weight) gw = at::empty({channels}, options);
@@ -302,7 +302,7 @@ class GroupNormActFunction : public torch::autograd::Function<GroupNormActFuncti
         using A = decltype(api);
         using P = typename A::P;
         using S = typename A::S;
-        const size_t bytes = A::norm_workspace(n, t, channels, ctx->saved_data["groups"].toInt());
+        const size_t bytes = A::norm_workspace(n, t, channels, ctx->saved_data["groups"].toInt(), 1);
         const Tensor ws = bytes > 0 ? at::empty({static_cast<int64_t>(bytes)}, input.options().dtype(at::kByte)) : Tensor();
         return A::norm_backward(ptr<P>(x), x.stride(0), x.stride(1), ptr<S>(w), ptr<S>(b), ptr<S>(stats), lens_ptr(lens), n,
                                 t, channels, ctx->saved_data["groups"].toInt(),
@@ -310,8 +310,8 @@ class GroupNormActFunction : public torch::autograd::Function<GroupNormActFuncti
                                 ptr<P>(gx), gx.stride(0), gx.stride(1), ptr<S>(gw), ptr<S>(gb), ptr<void>(ws), bytes,
                                 current_stream(input));
       }), c);
-      if (weight) gw = gw.to(weight->scalar_type());
-      if (bias) gb = gb.to(bias->scalar_type());
+      if (weight && gw.scalar_type() != weight->scalar_type()) gw = gw.to(weight->scalar_type());
+      if (bias && gb.scalar_type() != bias->scalar_type()) gb = gb.to(bias->scalar_type());
     }
     return once_differentiable("group_norm_act", {gx, Tensor(), gw, gb, Tensor(), Tensor(), Tensor()});
   }

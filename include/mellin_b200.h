@@ -356,10 +356,12 @@ int mellin_gated_recurrence_backward_bf16(const void *x, int64_t x_sn, int64_t x
 /* Group norm and an activation: y = act((x - mean) * rstd * weight[c] + bias[c]); mean and biased variance over an
  * utterance's frames and the channels / groups adjacent channels of a group, rstd = 1 / sqrt(var + eps).  weight / bias:
  * (channels), or NULL: ones / zeros.  act: 0 none, 1 ReLU, 2 SiLU (z sigmoid(z)), 3 GELU (z Phi(z)).  stats: receives
- * (batch, groups, 2) mean and rstd for backward, or NULL.  workspace: mellin_group_norm_act_workspace_bytes_*() bytes,
- * 16-byte aligned, for either call; its contents are clobbered.  Backward: grad_weight / grad_bias (channels) may be
+ * (batch, groups, 2) mean and rstd for backward, or NULL.  workspace: mellin_group_norm_act_workspace_bytes_*() bytes
+ * (backward: 0 for a forward call, 1 for a backward call), 16-byte aligned; NULL where that is 0.  Its contents are
+ * clobbered.  Backward: grad_weight / grad_bias (channels) may be
  * NULL; they are summed in a fixed order. */
-size_t mellin_group_norm_act_workspace_bytes_f32(int64_t batch, int64_t frames, int64_t channels, int64_t groups);
+size_t mellin_group_norm_act_workspace_bytes_f32(int64_t batch, int64_t frames, int64_t channels, int64_t groups,
+                                                 int backward);
 int mellin_group_norm_act_f32(const float *x, int64_t x_sn, int64_t x_st, const float *weight, const float *bias,
                               const int *lens, int64_t batch, int64_t frames, int64_t channels, int64_t groups,
                               double eps, int act, float *y, int64_t y_sn, int64_t y_st, float *stats, void *workspace,
@@ -370,7 +372,8 @@ int mellin_group_norm_act_backward_f32(const float *x, int64_t x_sn, int64_t x_s
                                        int64_t grad_y_sn, int64_t grad_y_st, float *grad_x, int64_t grad_x_sn,
                                        int64_t grad_x_st, float *grad_weight, float *grad_bias, void *workspace,
                                        size_t workspace_bytes, void *stream);
-size_t mellin_group_norm_act_workspace_bytes_f64(int64_t batch, int64_t frames, int64_t channels, int64_t groups);
+size_t mellin_group_norm_act_workspace_bytes_f64(int64_t batch, int64_t frames, int64_t channels, int64_t groups,
+                                                 int backward);
 int mellin_group_norm_act_f64(const double *x, int64_t x_sn, int64_t x_st, const double *weight, const double *bias,
                               const int *lens, int64_t batch, int64_t frames, int64_t channels, int64_t groups,
                               double eps, int act, double *y, int64_t y_sn, int64_t y_st, double *stats, void *workspace,
@@ -381,7 +384,8 @@ int mellin_group_norm_act_backward_f64(const double *x, int64_t x_sn, int64_t x_
                                        int64_t grad_y_sn, int64_t grad_y_st, double *grad_x, int64_t grad_x_sn,
                                        int64_t grad_x_st, double *grad_weight, double *grad_bias, void *workspace,
                                        size_t workspace_bytes, void *stream);
-size_t mellin_group_norm_act_workspace_bytes_f16(int64_t batch, int64_t frames, int64_t channels, int64_t groups);
+size_t mellin_group_norm_act_workspace_bytes_f16(int64_t batch, int64_t frames, int64_t channels, int64_t groups,
+                                                 int backward);
 int mellin_group_norm_act_f16(const void *x, int64_t x_sn, int64_t x_st, const float *weight, const float *bias,
                               const int *lens, int64_t batch, int64_t frames, int64_t channels, int64_t groups,
                               double eps, int act, void *y, int64_t y_sn, int64_t y_st, float *stats, void *workspace,
@@ -392,7 +396,8 @@ int mellin_group_norm_act_backward_f16(const void *x, int64_t x_sn, int64_t x_st
                                        int64_t grad_y_sn, int64_t grad_y_st, void *grad_x, int64_t grad_x_sn,
                                        int64_t grad_x_st, float *grad_weight, float *grad_bias, void *workspace,
                                        size_t workspace_bytes, void *stream);
-size_t mellin_group_norm_act_workspace_bytes_bf16(int64_t batch, int64_t frames, int64_t channels, int64_t groups);
+size_t mellin_group_norm_act_workspace_bytes_bf16(int64_t batch, int64_t frames, int64_t channels, int64_t groups,
+                                                 int backward);
 int mellin_group_norm_act_bf16(const void *x, int64_t x_sn, int64_t x_st, const float *weight, const float *bias,
                               const int *lens, int64_t batch, int64_t frames, int64_t channels, int64_t groups,
                               double eps, int act, void *y, int64_t y_sn, int64_t y_st, float *stats, void *workspace,

@@ -94,8 +94,10 @@ def test_entry_points_validate_before_touching_the_device(sfx):
     assert call(2, 4, 6, 4) == BAD and b"groups" in lib.mellin_last_error()
     assert call(2, 4, 6, 0) == BAD and call(2, 4, 6, 3, act=7) == BAD
     assert call(0, 4, 6, 3) == 0
-    if getattr(lib, "mellin_group_norm_act_workspace_bytes" + sfx)(2, 4, 6, 3):
-        assert call(2, 4, 6, 3) == WORKSPACE and b"workspace" in lib.mellin_last_error()
+    size = getattr(lib, "mellin_group_norm_act_workspace_bytes" + sfx)
+    assert size(2, 4, 6, 3, 0) == 0 and call(2, 4, 6, 3) == BAD and b"null pointer" in lib.mellin_last_error()
+    assert size(1, 9000, 8192, 1, 0) > 0 and call(1, 9000, 8192, 1) == WORKSPACE and b"workspace" in lib.mellin_last_error()
+    assert size(-1, 4, 6, 3, 1) == 0 and size(2, 4, 6, 4, 1) == 0
     drop = getattr(lib, "mellin_philox_dropout" + sfx)
 
     def dropout(rows, cols, p):
