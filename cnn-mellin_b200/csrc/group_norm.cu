@@ -82,7 +82,7 @@ struct NormArgs {
   Acc<T> eps = 0;
   // the fused kernels
   int team = 0, col_ranks = 1, row_ranks = 1;  // threads that share a group in a block; blocks of a cluster across both
-  int team_log2 = 0, across = 1, packs = 1, rows = 1;  // blocks across the groups, packs of a frame, frames of a team
+  int team_log2 = 0, packs = 1, rows = 1;  // packs of a frame, frames of a team
   unsigned packs_magic = 0;                            // ceil(2^20 / packs)
   int kept = 0;                                // most frames of a thread in shared memory
   int per_block = 1;                           // utterances a backward block takes one after the other
@@ -111,34 +111,27 @@ __device__ __forceinline__ void join(A &mean, A &m2, A &count, A mean_b, A m2_b,
 // to its own slots in shared memory, all copies issued at once, so x (and grad_y) is read from HBM once.  Frames beyond
 // those are read again for the result, from L2 as a rule.  Teams are as small as the group allows, down to four threads,
 // so that groups of a single frame share a warp.  Bound by HBM: two or more blocks a multiprocessor overlap one's sums
-// with another's loads and stores.  (Kept in registers instead, 64 a thread, float32 at 32 x 200..800 x
-// 1024 took 68 us forward and 151 us backward against 39 and 61: fewer bytes in flight, more clusters, code beyond the
-// instruction cache.)
+// with another's loads and stores.  Measured with 32 utterances of 200 to 800 frames, 1024 channels, 32 groups: float32
+// and ReLU 37 us forward and 55 us backward (bytes alone: 26 and 36), bfloat16 and SiLU 27 and 47 (13 and 18: the special
+// function unit and the conversions count there).  Values kept in registers instead, 64 a thread: 68 and 151 us (fewer
+// bytes in flight, more clusters, code beyond the instruction cache).  Utterances are taken as they come: sorting them
+// costs every block more than the shorter tail gains (float32 backward 60 us).
 
 struct Seat {  // a thread's place
   int n, len, g, c, rank, size, team_id, j, tx, ty, rows, row_rank, cols;
   bool some, live;  // there are columns for this rank; this thread has one
 };
 template <typename T, int V>
-__device__ __forceinline__ Seat seat_of(const NormArgs<T> &a, bool sorted) {
+__device__ __forceinline__ Seat seat_of(const NormArgs<T> &a) {
   Seat s;
-  s.size = a.col_ranks * a.row_ranks, s.rank = 0;
-  unsigned block = blockIdx.x, col_rank = 0;
-  s.row_rank = 0;
-  if (s.size > 1) {
-    s.rank = (int)(block % (unsigned)s.size), block /= (unsigned)s.size;
-    s.row_rank = s.rank, col_rank = 0;
-    if (a.col_ranks > 1) s.row_rank = s.rank / a.col_ranks, col_rank = (unsigned)s.rank % a.col_ranks;
-  }
-  const unsigned turn = a.across == 1 ? block : block / (unsigned)a.across;
-  if (sorted) {
-    const Utterance u = utterance_of(a.lens, a.batch, a.frames, (int)turn);
-    s.n = u.n, s.len = u.len;
-  } else {
-    s.n = (int)turn, s.len = 0;
-  }
+  s.size = a.col_ranks * a.row_ranks;  // powers of two
+  s.rank = (int)(blockIdx.x & (s.size - 1));
+  s.row_rank = s.rank >> (31 - __clz(a.col_ranks));
+  const unsigned col_rank = s.rank & (a.col_ranks - 1), block = blockIdx.x >> (31 - __clz(s.size));
+  const unsigned turn = blockIdx.z * 65535u + blockIdx.y;
+  s.n = (int)turn, s.len = a.per_block == 1 && s.n < a.batch ? live_frames(a.lens, s.n, a.frames) : 0;
   s.team_id = (int)(threadIdx.x >> a.team_log2), s.j = (int)(threadIdx.x & ((1u << a.team_log2) - 1));
-  s.g = (int)((block - turn * a.across) * (kThreads >> a.team_log2)) + s.team_id;
+  s.g = (int)(block * (kThreads >> a.team_log2)) + s.team_id;
   s.cols = a.packs, s.rows = a.rows, s.some = true;
   if (a.col_ranks > 1) {
     const int left = a.packs - (int)col_rank * a.team;  // none for the last ranks where the ranks are not a multiple
@@ -211,31 +204,38 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 
 // Sum over a team, the same bits in all its threads; `slots` (one a warp) is not used again before the next block barrier
 // but one.
-template <typename A>
-__device__ __forceinline__ A team_sum(A v, const Seat &s, int team, A *slots) {
+template <typename A, int Q>
+__device__ __forceinline__ void team_sum(A (&v)[Q], const Seat &s, int team, A (*slots)[kThreads / 32]) {
 #pragma unroll
-  for (int o = 1; o < 32; o *= 2) {
-    const A other = __shfl_xor_sync(0xffffffffu, v, o);
-    if (o < team) v += other;
-  }
+  for (int o = 1; o < 32; o *= 2)
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const A other = __shfl_xor_sync(0xffffffffu, v[q], o);
+      if (o < team) v[q] += other;
+    }
   if (team > 32) {
-    if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) slots[q][threadIdx.x >> 5] = v[q];
+    }
     __syncthreads();
-    if (team == kThreads) {
-      A all[kThreads / 32];
 #pragma unroll
-      for (int i = 0; i < kThreads / 32; ++i) all[i] = slots[i];
+    for (int q = 0; q < Q; ++q) {
+      if (team == kThreads) {
+        A all[kThreads / 32];
 #pragma unroll
-      for (int o = kThreads / 64; o > 0; o /= 2)
+        for (int i = 0; i < kThreads / 32; ++i) all[i] = slots[q][i];
 #pragma unroll
-        for (int i = 0; i < o; ++i) all[i] += all[i + o];
-      v = all[0];
-    } else {
-      v = 0;
-      for (int i = 0; i < team / 32; ++i) v += slots[s.team_id * (team / 32) + i];
+        for (int o = kThreads / 64; o > 0; o /= 2)
+#pragma unroll
+          for (int i = 0; i < o; ++i) all[i] += all[i + o];
+        v[q] = all[0];
+      } else {
+        v[q] = 0;
+        for (int i = 0; i < team / 32; ++i) v[q] += slots[q][s.team_id * (team / 32) + i];
+      }
     }
   }
-  return v;
 }
 
 template <typename T, int V, int MB>
@@ -244,7 +244,8 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_kernel(const NormArgs
   extern __shared__ __align__(16) unsigned char shared_raw[];
   __shared__ __align__(16) A slots[2][kThreads / 32];
   __shared__ A ranks[kMaxRanks][3];
-  const Seat s = seat_of<T, V>(a, true);
+  const Seat s = seat_of<T, V>(a);
+  if (s.n >= a.batch) return;  // the last plane of the grid is not full
   if (s.size > 1) cluster_arrive();
   const int len = s.len;
   const Span span = span_of(len, s.row_rank, a.row_ranks);
@@ -269,10 +270,13 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_kernel(const NormArgs
 
   // the block's: sum of the values, then of the squared deviations from their mean
   A count = A(span.end - span.begin) * A(s.some ? s.cols * V : 0);
-  const A total = team_sum<A>(m.count * m.mean, s, a.team, slots[0]);
-  A mean = count > A(0) ? total / count : A(0);
+  A total[1] = {m.count * m.mean};
+  team_sum(total, s, a.team, &slots[0]);
+  A mean = count > A(0) ? total[0] / count : A(0);
   const A d = m.mean - mean;
-  A m2 = team_sum<A>(m.m2 + m.count * d * d, s, a.team, slots[1]);
+  A squares[1] = {m.m2 + m.count * d * d};
+  team_sum(squares, s, a.team, &slots[1]);
+  A m2 = squares[0];
   if (s.size > 1) {
     auto cluster = cooperative_groups::this_cluster();
     cluster_wait();  // no block writes to one that has not started
@@ -333,10 +337,11 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_backward_kernel(const
   extern __shared__ __align__(16) unsigned char shared_raw[];
   __shared__ __align__(16) A slots[2][2][kThreads / 32];
   __shared__ A ranks[2][kMaxRanks][2];
-  const Seat s = seat_of<T, V>(a, !MANY);
-  // with one utterance a block, `chunk` is that utterance, longest first; else the first of a run in order
+  const Seat s = seat_of<T, V>(a);
+  // with one utterance a block, `chunk` is that utterance, else a run of them
   const long long chunk = s.n, n_first = MANY ? chunk * a.per_block : chunk;
   const long long n_end = MANY ? min(n_first + a.per_block, (long long)a.batch) : n_first + 1;
+  if (n_first >= a.batch) return;  // the last plane of the grid is not full
   if (s.size > 1) cluster_arrive();
   bool met = false;
   A weight[V], bias[V], p1[V], p2[V];
@@ -361,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_backward_kernel(const
       copy_async<T, V>(mine_y + i * (kThreads * V), from_y);
     }
     if (s.live) clear_from<T, V>(a.grad_x, n, s.c, len + s.row_rank * s.rows + s.ty, a.row_ranks * s.rows, a.frames);
-    A mean = 0, rstd = 0, scale[V], q1[V], q2[V], s1 = 0, s2 = 0;
+    A mean = 0, rstd = 0, scale[V], q1[V], q2[V], sums[2] = {A(0), A(0)};
     if (s.live) mean = a.stats[(n * a.groups + s.g) * 2], rstd = a.stats[(n * a.groups + s.g) * 2 + 1];
 #pragma unroll
     for (int v = 0; v < V; ++v) q1[v] = q2[v] = 0, scale[v] = rstd * weight[v];
@@ -385,9 +390,10 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_backward_kernel(const
       q2[v] *= rstd;  // of gz * xhat
       if constexpr (MANY) p1[v] += q1[v], p2[v] += q2[v];
       else p1[v] = q1[v], p2[v] = q2[v];
-      s1 += weight[v] * q1[v], s2 += weight[v] * q2[v];
+      sums[0] += weight[v] * q1[v], sums[1] += weight[v] * q2[v];
     }
-    s1 = team_sum<A>(s1, s, a.team, slots[buffer][0]), s2 = team_sum<A>(s2, s, a.team, slots[buffer][1]);
+    team_sum(sums, s, a.team, slots[buffer]);
+    A s1 = sums[0], s2 = sums[1];
     if (s.size > 1) {
       auto cluster = cooperative_groups::this_cluster();
       if (!met) cluster_wait();
@@ -792,7 +798,7 @@ int prepare(const char *who, NormArgs<T> &a, int64_t batch, int64_t frames, int6
   if (groups <= 0 || channels % groups != 0)
     return fail(MELLIN_ERR_BAD_ARGUMENT, std::string(who) + ": the channels are not a multiple of the groups");
   if (act < kNone || act > kGelu) return fail(MELLIN_ERR_BAD_ARGUMENT, std::string(who) + ": unknown activation");
-  if (batch * std::max(groups, channels) > 0x7fffffffLL)
+  if (batch * std::max(groups, channels) > 0x7fffffffLL || batch > 0x7fff0000LL)
     return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many utterances times channels");
   a.batch = (int)batch, a.frames = (int)frames, a.channels = (int)channels, a.groups = (int)groups, a.act = act;
   if (batch == 0 || channels == 0) return MELLIN_OK;
@@ -820,10 +826,14 @@ long long grid_for(NormArgs<T> &a, int V) {
 }
 
 template <typename K, typename T>
-int launch(const char *who, K kernel, const NormArgs<T> &a, long long blocks, int cluster, size_t shared, cudaStream_t st) {
+int launch(const char *who, K kernel, const NormArgs<T> &a, long long blocks, int cluster, size_t shared, cudaStream_t st,
+           long long utterances = 1) {
   if (blocks > 0x7fffffffLL) return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many blocks");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks), cfg.blockDim = dim3(kThreads), cfg.stream = st, cfg.dynamicSmemBytes = shared;
+  const unsigned planes = (unsigned)((utterances + 65534) / 65535);  // the grid's second extent ends at 65535
+  cfg.gridDim = dim3((unsigned)blocks, (unsigned)std::min<long long>(utterances, 65535), planes);
+  if (planes > 65535) return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many blocks");
+   cfg.blockDim = dim3(kThreads), cfg.stream = st, cfg.dynamicSmemBytes = shared;
   if (shared > 44 * 1024) {  // with the static arrays beside it: beyond what a launch may have without asking
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 4096);
     if (err != cudaSuccess) return fail(MELLIN_ERR_LAUNCH, std::string(who) + ": " + cudaGetErrorString(err));
@@ -850,16 +860,14 @@ void take_plan(NormArgs<T> &a, const FusedPlan &p, int V) {
   a.team = p.team, a.col_ranks = p.col_ranks, a.row_ranks = p.row_ranks, a.kept = p.kept;
   a.team_log2 = 0;
   while ((1 << a.team_log2) < p.team) ++a.team_log2;
-  const int teams = kThreads / p.team;
-  a.across = (a.groups + teams - 1) / teams;
   a.packs = a.channels / a.groups / V, a.rows = std::max(1, p.team / a.packs);
   a.packs_magic = ((1u << 20) + a.packs - 1) / a.packs;
 }
 template <typename T, int V, int MB>
 int launch_fused(const char *who, NormArgs<T> a, const FusedPlan &p, cudaStream_t st) {
   take_plan(a, p, V);
-  return launch(who, norm_fused_kernel<T, V, MB>, a, a.batch * p.blocks_per_utterance, p.col_ranks * p.row_ranks,
-                (size_t)p.kept * kThreads * V * sizeof(T), st);
+  return launch(who, norm_fused_kernel<T, V, MB>, a, p.blocks_per_utterance, p.col_ranks * p.row_ranks,
+                (size_t)p.kept * kThreads * V * sizeof(T), st, a.batch);
 }
 template <typename T, int V, int MB>
 int launch_fused_backward(const char *who, NormArgs<T> &a, const FusedPlan &p, cudaStream_t st) {
@@ -868,9 +876,10 @@ int launch_fused_backward(const char *who, NormArgs<T> &a, const FusedPlan &p, c
   const long long chunks = (a.batch + a.per_block - 1) / a.per_block;
   a.parts = (int)(chunks * p.row_ranks);
   const size_t shared = std::max((size_t)p.kept * kThreads * V * sizeof(T) * 2, kThreads * V * 2 * sizeof(Acc<T>));
-  const long long blocks = chunks * p.blocks_per_utterance;
-  if (a.per_block == 1) return launch(who, norm_fused_backward_kernel<T, V, MB, false>, a, blocks, p.col_ranks * p.row_ranks, shared, st);
-  return launch(who, norm_fused_backward_kernel<T, V, MB, true>, a, blocks, p.col_ranks * p.row_ranks, shared, st);
+  const int cluster = p.col_ranks * p.row_ranks;
+  if (a.per_block == 1)
+    return launch(who, norm_fused_backward_kernel<T, V, MB, false>, a, p.blocks_per_utterance, cluster, shared, st, chunks);
+  return launch(who, norm_fused_backward_kernel<T, V, MB, true>, a, p.blocks_per_utterance, cluster, shared, st, chunks);
 }
 
 template <typename T>

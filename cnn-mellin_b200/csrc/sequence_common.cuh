@@ -65,7 +65,7 @@ struct Utterance {
 };
 __device__ __forceinline__ Utterance utterance_of(const int *lens, int batch, int frames, int turn) {
   if (lens == nullptr) return {turn, frames};
-  if (batch > 32 || batch == 1) return {turn, live_frames(lens, turn, frames)};
+  if (batch > 32 || batch == 1) return {turn, turn < batch ? live_frames(lens, turn, frames) : 0};
   const int lane = threadIdx.x & 31, mine = lane < batch ? lens[lane] : INT_MIN;
   int place = 0;
 #pragma unroll

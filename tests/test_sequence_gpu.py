@@ -316,6 +316,28 @@ def test_group_norm_other_shapes():
         assert all(torch.equal(g, torch.zeros_like(g)) for g in grads)
 
 
+def test_many_utterances():
+    """More utterances than a grid's second extent has blocks, and than fit one block's run: the same bits as in pieces."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn(140001, 1, 16, device="cuda", generator=gen, requires_grad=True)
+    gy = torch.randn(140001, 1, 16, device="cuda", generator=gen)
+    w = torch.randn(16, device="cuda", generator=gen, requires_grad=True)
+    y = sequence.group_norm_act(x, 2, w, activation="silu")
+    gx, gw = torch.autograd.grad(y, [x, w], gy)
+    want_w = torch.zeros(16, dtype=torch.float64, device="cuda")
+    for part in range(0, 140001, 40000):
+        piece = x.detach()[part:part + 40000].requires_grad_(True)
+        z = sequence.group_norm_act(piece, 2, w, activation="silu")
+        g, v = torch.autograd.grad(z, [piece, w], gy[part:part + 40000])
+        assert torch.equal(z, y[part:part + 40000]) and torch.equal(g, gx[part:part + 40000])
+        want_w += v
+    # sums of 140001 terms of order one in float32, in other groupings: 2^-24 * 140001 relative to the terms' sum at worst
+    assert float((gw - want_w).abs().max()) <= 140001 * 2 ** -24 * 140001 ** 0.5 * 4
+    h, _ = sequence.gated_recurrence(x.detach().expand(140001, 9, 16), gy.expand(140001, 9, 16))
+    h2, _ = sequence.gated_recurrence(x.detach()[139000:].expand(1001, 9, 16), gy[139000:].expand(1001, 9, 16))
+    assert torch.equal(h[139000:], h2)
+
+
 def test_group_norm_strides_beyond_32_bits():
     flat = torch.zeros(5 * 2 ** 30 + 64, dtype=torch.bfloat16, device="cuda")
     x = flat.as_strided((1, 6, 32), (0, 2 ** 30, 1))
