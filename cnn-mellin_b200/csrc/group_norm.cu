@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_kernel(const NormArgs
     for (int i = 1; i < s.size; ++i) join(mean, m2, count, ranks[i][0], ranks[i][1], ranks[i][2]);
   }
   if (!s.live) return;
-  const A rstd = A(1) / sqrt((count > A(0) ? m2 / count : A(0)) + a.eps);
+  const A rstd = count > A(0) ? A(1) / sqrt(m2 / count + a.eps) : A(0);  // no frames: nothing to scale, no 0 * inf
   if (a.stats_out != nullptr && s.j == 0 && s.rank == 0) {
     A *out = a.stats_out + (s.n * a.groups + s.g) * 2;
     out[0] = mean, out[1] = rstd;
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(kThreads) norm_stats_kernel(const NormArgs<T> 
   }
   if (threadIdx.x == 0) {
     a.stats_out[2 * (long long)blockIdx.x] = mean;
-    a.stats_out[2 * (long long)blockIdx.x + 1] = A(1) / sqrt((count > A(0) ? m2 / count : A(0)) + a.eps);
+    a.stats_out[2 * (long long)blockIdx.x + 1] = count > A(0) ? A(1) / sqrt(m2 / count + a.eps) : A(0);
   }
 }
 

@@ -284,12 +284,12 @@ inline int launched(const char *who) {
   return MELLIN_OK;
 }
 
-// Extents of a (batch, frames, channels) tensor the kernels index: non-negative, the product below 2^62, batch and
-// channels below 2^31, frames at most 2^30 (coordinates are 32-bit, a step past the end included; offsets are 64-bit).
+// Extents of a (batch, frames, channels) tensor the kernels index: non-negative, the product below 2^62, batch below
+// 2^31, frames and channels at most 2^30 (coordinates are 32-bit, a step past the end included; offsets are 64-bit).
 inline int check_extents(const char *who, int64_t batch, int64_t frames, int64_t channels) {
   if (batch < 0 || frames < 0 || channels < 0) return fail(MELLIN_ERR_BAD_ARGUMENT, std::string(who) + ": negative extent");
-  if (batch > 0x7fffffffLL || frames > 0x40000000LL || channels > 0x7fffffffLL)
-    return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": batch or channels above 2^31 - 1, or frames above 2^30");
+  if (batch > 0x7fffffffLL || frames > 0x40000000LL || channels > 0x40000000LL)
+    return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": batch above 2^31 - 1, or frames or channels above 2^30");
   if ((long double)batch * (long double)frames * (long double)channels > 4.0e18L)
     return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": more than 2^62 elements");
   return MELLIN_OK;

@@ -47,7 +47,8 @@ def gated_recurrence(
     their outputs and gradients are zero.  ``reverse``: from an utterance's last frame to its first.  ``initial``
     (batch, channels) is the state before the first frame met, zeros when not given; ``final`` the state after the last
     one met, float32 (float64 for float64 input) whatever the input's type, so that a stream fed in pieces, down to one
-    frame a call, carries it unrounded.  Differentiable in input, gate and initial."""
+    frame a call, carries it unrounded.  The frames are joined in runs, so an infinite value makes those after it infinite
+    or NaN.  Differentiable in input, gate and initial."""
     _on_device("gated_recurrence", input)
     return torch.ops.mellin.gated_recurrence(input, gate, initial, lens, reverse)
 
@@ -96,9 +97,7 @@ def philox_dropout(
         return input if residual is None else torch.ops.mellin.philox_dropout(input, 0.0, 0, None, residual)
     if isinstance(seed, torch.Tensor):
         return torch.ops.mellin.philox_dropout(input, p, 0, seed, residual)
-    if seed is None:
-        seed = int(torch.randint(0, 2 ** 62, (1,)).item())
-    seed &= (1 << 64) - 1
+    seed = int(torch.randint(0, 2 ** 62, (1,)).item()) if seed is None else int(seed) & ((1 << 64) - 1)
     return torch.ops.mellin.philox_dropout(input, p, seed - (1 << 64) if seed >> 63 else seed, None, residual)
 
 

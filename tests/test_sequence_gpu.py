@@ -484,20 +484,23 @@ def test_refusals():
         y.sum().backward()
 
 
-def test_other_stream_and_captured_graph():
-    """The same results on a stream of the caller's, and from a graph that is replayed on other inputs."""
-    lens = torch.tensor([40, 0, 25], dtype=torch.int32, device="cuda")
+@pytest.mark.parametrize("frames", [3, 40, 2600])
+def test_other_stream_and_captured_graph(frames):
+    """The same results on a stream of the caller's, and from a graph that is replayed on other inputs: at a few frames, at
+    sizes that one block has, and at sizes that clusters share and whose parameter sums are added by a dependent kernel."""
+    lens = torch.tensor([frames, 0, frames * 5 // 8], dtype=torch.int32, device="cuda")
     gen = torch.Generator(device="cuda").manual_seed(8)
-    w, b = torch.randn(32, device="cuda", generator=gen), torch.randn(32, device="cuda", generator=gen)
+    w, b = (torch.randn(32, device="cuda", generator=gen).requires_grad_(True) for _ in range(2))
     seed = torch.tensor(1, device="cuda")
-    x = torch.randn(3, 40, 64, device="cuda", generator=gen)
+    x = torch.randn(3, frames, 64, device="cuda", generator=gen)
 
     def step(x):
         x = x.detach().requires_grad_(True)
         y, final = sequence.gated_recurrence(x, lens=lens)
         z = sequence.group_norm_act(y, 4, w, b, lens, activation="silu")
         out = sequence.philox_dropout(z, 0.2, True, seed, y)
-        return [out, final] + list(torch.autograd.grad([out, final], [x], [torch.ones_like(out), torch.ones_like(final)]))
+        return [out.detach(), final.detach()] + list(
+            torch.autograd.grad([out, final], [x, w, b], [torch.ones_like(out), torch.ones_like(final)]))
 
     eager = step(x)
     side = torch.cuda.Stream()
@@ -514,10 +517,51 @@ def test_other_stream_and_captured_graph():
     for k in range(3):
         static.copy_(x * (k + 1))
         seed.fill_(k + 1)
-        lens.copy_(torch.tensor([40 - k, k, 25], dtype=torch.int32))
+        lens.copy_(torch.tensor([frames - k, k, frames // 2], dtype=torch.int32))
         graph.replay()
         want = step(x * (k + 1))
         assert all(torch.equal(a, c) for a, c in zip(captured, want)), k
+
+
+def test_entry_points_with_strides_of_the_callers():
+    """The C ABI from raw pointers: time running backwards through a negative stride, states off the 16-byte grid."""
+    import ctypes
+
+    lib, i64, ptr = capi.lib(), ctypes.c_int64, ctypes.c_void_p
+    stream = ptr(torch.cuda.current_stream().cuda_stream)
+    for frames in (3, 70, 300):
+        n, c = 2, 16
+        gen = torch.Generator(device="cuda").manual_seed(frames)
+        x, gate, gy = (torch.randn(n, frames, c, device="cuda", generator=gen) for _ in range(3))
+        lib.mellin_gated_recurrence_state_count.restype = i64
+        count = lib.mellin_gated_recurrence_state_count(i64(n), i64(frames), i64(c))
+        y, final = torch.empty_like(x), torch.empty(n, c, device="cuda")
+        states = torch.empty(count + 1, device="cuda")[1:]
+        last = (frames - 1) * c * 4
+
+        def at(t):
+            return [ptr(t.data_ptr() + last), i64(frames * c), i64(-c)]
+
+        assert lib.mellin_gated_recurrence_f32(*at(x), *at(gate), ptr(0), ptr(0), 0, i64(n), i64(frames), i64(c), *at(y),
+                                               ptr(final.data_ptr()), ptr(states.data_ptr()), stream) == 0
+        xs, gs = x.clone().requires_grad_(True), gate.clone().requires_grad_(True)
+        want, want_final = sequence.gated_recurrence(xs, gs, reverse=True)
+        want_x, want_g = torch.autograd.grad(want, [xs, gs], gy)
+        gx, gg = torch.empty_like(x), torch.empty_like(x)
+        assert lib.mellin_gated_recurrence_backward_f32(
+            *at(x), *at(gate), ptr(states.data_ptr()), ptr(0), 0, i64(n), i64(frames), i64(c), *at(gy), ptr(0), *at(gx),
+            *at(gg), ptr(0), stream) == 0
+        # other forms of the same sums: a few units of values of order one to four
+        for got, ref in ((y, want), (final, want_final), (gx, want_x), (gg, want_g)):
+            assert float((got - ref).detach().abs().max()) <= 1e-5
+
+
+def test_group_norm_without_epsilon():
+    """eps = 0 and an utterance without a frame: nothing of it reaches the parameters' gradients."""
+    x = torch.randn(3, 9, 8, device="cuda", requires_grad=True)
+    w, b = torch.ones(8, device="cuda", requires_grad=True), torch.zeros(8, device="cuda", requires_grad=True)
+    y = sequence.group_norm_act(x, 2, w, b, torch.tensor([9, 0, 4], dtype=torch.int32, device="cuda"), 0.0, "silu")
+    assert all(torch.isfinite(g).all() for g in torch.autograd.grad(y.sum(), [x, w, b])) and torch.isfinite(y).all()
 
 
 def test_autocast_meets_in_the_wider_type():
