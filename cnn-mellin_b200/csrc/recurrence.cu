@@ -794,12 +794,15 @@ int run(const char *who, RecurrenceArgs<T> a, int64_t batch, int64_t frames, int
       return launch_long<T, 1, 16, BACKWARD>(who, a, stream);
     }
     // V, CL, W and blocks a multiprocessor, measured at 32 utterances of 200 to 800 frames and 1024 channels (us, forward
-    // / backward): 16 bits <4, 16, 8, 2> 30 / 66, <4, 8, 4, 4> 32 / 47, <2, 16, 4, 4> 35 / 49; float <4, 8, 4, 4> 45 / 78,
-    // <4, 8, 4, 3> 51 / 76, <2, 16, 4, 4> 45 / 80.
+    // / backward): 16 bits <4, 16, 4, 4> 30 / 73, <4, 16, 4, 2> 35 / 47, <4, 8, 4, 4> 31 / 47, <4, 16, 8, 2> 29 / 66 (39
+    // against 35 forward where all have 800 frames); float <4, 8, 4, 4> 44 / 78, <4, 8, 4, 3> 50 / 77, <4, 16, 4, 2>
+    // 45 / 71.  Bytes alone: 18 / 31 and 36 / 62.  What is left goes to the joins (a barrier every step), to 26
+    // instructions an element, and to 3.5 blocks a multiprocessor; packed multiply-adds changed nothing.
     constexpr int V = sizeof(T) == 8 ? 2 : 4;
     if (!packed(a, channels, V)) return launch_scan<T, 1, 32, 4, BACKWARD ? 3 : 4, BACKWARD>(who, a, stream);
-    if constexpr (sizeof(T) == 2 && !BACKWARD) return launch_scan<T, V, 16, 8, 2, BACKWARD>(who, a, stream);
-    else return launch_scan<T, V, 8, 4, sizeof(T) == 2 || !BACKWARD ? 4 : 3, BACKWARD>(who, a, stream);
+    if constexpr (sizeof(T) == 2 && !BACKWARD) return launch_scan<T, V, 16, 4, 4, BACKWARD>(who, a, stream);
+    else if constexpr (sizeof(T) == 4 && BACKWARD) return launch_scan<T, V, 16, 4, 2, BACKWARD>(who, a, stream);
+    else return launch_scan<T, V, 8, 4, 4, BACKWARD>(who, a, stream);
   });
 }
 
