@@ -799,7 +799,11 @@ int run(const char *who, RecurrenceArgs<T> a, int64_t batch, int64_t frames, int
     // 45 / 71.  Bytes alone: 18 / 31 and 36 / 62.  What is left goes to the joins (a barrier every step), to 26
     // instructions an element, and to 3.5 blocks a multiprocessor; packed multiply-adds changed nothing.
     constexpr int V = sizeof(T) == 8 ? 2 : 4;
-    if (!packed(a, channels, V)) return launch_scan<T, 1, 32, 4, BACKWARD ? 3 : 4, BACKWARD>(who, a, stream);
+    if (!packed(a, channels, V)) {
+      // an even number of channels: pairs, bfloat16 33 / 49; else one by one, 41 / 86
+      if (V > 2 && packed(a, channels, 2)) return launch_scan<T, 2, 16, 4, 4, BACKWARD>(who, a, stream);
+      return launch_scan<T, 1, 32, 4, BACKWARD ? 3 : 4, BACKWARD>(who, a, stream);
+    }
     if constexpr (sizeof(T) == 2 && !BACKWARD) return launch_scan<T, V, 16, 4, 4, BACKWARD>(who, a, stream);
     else if constexpr (sizeof(T) == 4 && BACKWARD) return launch_scan<T, V, 16, 4, 2, BACKWARD>(who, a, stream);
     else return launch_scan<T, V, 8, 4, 4, BACKWARD>(who, a, stream);

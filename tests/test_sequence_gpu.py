@@ -87,6 +87,10 @@ RECURRENCES = [
     (2, 700, 72, [513, 700], False, True, "dense"),
     (1, 5000, 8, None, False, True, "packed"),
     (70, 9, 48, [i % 10 for i in range(70)], True, False, "packed"),
+    (3, 140, 34, [140, 139, 7], True, True, "dense"),
+    (2, 300, 50, None, False, True, "packed"),
+    (40, 300, 130, [300 - 7 * i for i in range(40)], False, True, "time-major"),
+    (33, 600, 160, [600] * 16 + [i for i in range(17)], True, False, "packed"),
 ]
 
 
