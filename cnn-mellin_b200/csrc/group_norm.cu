@@ -24,7 +24,6 @@ using namespace seq;
 
 constexpr int kThreads = 256;
 constexpr int kMaxRanks = 8;    // blocks of a cluster: the portable limit
-constexpr int kMaxChunks = 64;  // pieces of an utterance's frames in the kernels that pass over the tensor twice
 
 enum Activation { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3 };
 
@@ -82,16 +81,15 @@ struct NormArgs {
   Acc<T> eps = 0;
   // the fused kernels
   int team = 0, col_ranks = 1, row_ranks = 1;  // threads that share a group in a block; blocks of a cluster across both
-  int team_log2 = 0, packs = 1, rows = 1;  // packs of a frame, frames of a team
-  unsigned packs_magic = 0;                            // ceil(2^20 / packs)
+  int team_log2 = 0, packs = 1, rows = 1;      // packs of a group's frame, frames a block (team) has at a time
+  unsigned packs_magic = 0;                    // ceil(2^20 / packs of a frame in a block)
   int kept = 0;                                // most frames of a thread in shared memory
   int per_block = 1;                           // utterances a backward block takes one after the other
   int parts = 1;                               // sets of parameter sums: (parts, channels, 2) at `part`
-  // the kernels that pass over the tensor twice
-  Acc<T> *part = nullptr;    // (batch, chunks, channels, 2)
-  Acc<T> *sums = nullptr;    // (batch, channels, 2): P1, P2
-  Acc<T> *gsums = nullptr;   // (batch, groups, 2): sums of weight * P1, weight * P2, over M
-  int chunks = 0, tx = 0, slabs = 0;
+  // the kernels for large groups: `tx` packs of `slabs` blocks make a frame of a group, `chunks` of `chunk_rows` its frames
+  Acc<T> *part = nullptr;   // forward (batch, groups, entries, 3): mean, m2, count; backward (batch, chunks, channels, 2)
+  Acc<T> *gsums = nullptr;  // (batch, groups, entries, 2): sums of weight * P1, weight * P2
+  int chunks = 0, tx = 0, slabs = 0, chunk_rows = 0, entries = 0;
 };
 
 // (mean, sum of squared deviations, count) of two sets of values, joined
@@ -107,10 +105,9 @@ __device__ __forceinline__ void join(A &mean, A &m2, A &count, A mean_b, A m2_b,
 // ---- one pass: a group's values stay in shared memory between the sums and the result ---------------------------------
 //
 // `team` threads of a block (or the blocks of a cluster, team = all threads of each) share one utterance's group.  A
-// thread has V adjacent channels, always the same, of every `rows`-th frame; the first `kept` of its frames are copied
-// to its own slots in shared memory, all copies issued at once, so x (and grad_y) is read from HBM once.  Frames beyond
-// those are read again for the result, from L2 as a rule.  Teams are as small as the group allows, down to four threads,
-// so that groups of a single frame share a warp.  Bound by HBM: two or more blocks a multiprocessor overlap one's sums
+// thread has V adjacent channels, always the same, of every `rows`-th frame; these are copied to its own slots in shared
+// memory, all copies issued at once, so x (and grad_y) is read once.  Teams are as small as the group allows, down to
+// four threads, so that groups of a single frame share a warp.  Bound by HBM: two or more blocks a multiprocessor overlap one's sums
 // with another's loads and stores.  Measured with 32 utterances of 200 to 800 frames, 1024 channels, 32 groups: float32
 // and ReLU 37 us forward and 55 us backward (bytes alone: 26 and 36), bfloat16 and SiLU 27 and 47 (13 and 18: the special
 // function unit and the conversions count there).  Values kept in registers instead, 64 a thread: 68 and 151 us (fewer
@@ -174,28 +171,25 @@ template <typename A>
 struct Moments {
   A mean = 0, m2 = 0, count = 0;
 };
-constexpr int kBatch = 16;  // frames a thread takes into its moments together
-template <typename T, int V, typename F>
-__device__ __forceinline__ void add_frames(Moments<Acc<T>> &m, int frames, F &&frame) {
+// `n` (1 to B) frames
+template <typename T, int V, int B, typename F>
+__device__ __forceinline__ void add_batch(Moments<Acc<T>> &m, int n, F &&frame) {
   using A = Acc<T>;
-  for (int i0 = 0; i0 < frames; i0 += kBatch) {
-    A pivot = 0, sum = 0, squares = 0;
-    const int n = min(kBatch, frames - i0);
+  A pivot = 0, sum = 0, squares = 0;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (i < n) {
-        const Raw<T, V> r = frame(i0 + i);
-        if (i == 0) pivot = element(r, 0);
+  for (int i = 0; i < B; ++i) {
+    if (i < n) {
+      const Raw<T, V> r = frame(i);
+      if (i == 0) pivot = element(r, 0);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const A d = element(r, v) - pivot;
-          sum += d, squares += d * d;
-        }
+      for (int v = 0; v < V; ++v) {
+        const A d = element(r, v) - pivot;
+        sum += d, squares += d * d;
       }
     }
-    const A count = A(n * V), off = sum * reciprocal_unit(count);
-    join(m.mean, m.m2, m.count, pivot + off, max(squares - sum * off, A(0)), count);
   }
+  const A count = A(n * V), off = sum * reciprocal_unit(count);
+  join(m.mean, m.m2, m.count, pivot + off, max(squares - sum * off, A(0)), count);
 }
 
 // A cluster's barrier in two halves: what lies between them does not wait for blocks that have not started
@@ -205,7 +199,7 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // Sum over a team, the same bits in all its threads; `slots` (one a warp) is not used again before the next block barrier
 // but one.
 template <typename A, int Q>
-__device__ __forceinline__ void team_sum(A (&v)[Q], const Seat &s, int team, A (*slots)[kThreads / 32]) {
+__device__ __forceinline__ void team_sum(A (&v)[Q], int team_id, int team, A (*slots)[kThreads / 32]) {
 #pragma unroll
   for (int o = 1; o < 32; o *= 2)
 #pragma unroll
@@ -232,7 +226,7 @@ __device__ __forceinline__ void team_sum(A (&v)[Q], const Seat &s, int team, A (
         v[q] = all[0];
       } else {
         v[q] = 0;
-        for (int i = 0; i < team / 32; ++i) v[q] += slots[q][s.team_id * (team / 32) + i];
+        for (int i = 0; i < team / 32; ++i) v[q] += slots[q][team_id * (team / 32) + i];
       }
     }
   }
@@ -250,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_kernel(const NormArgs
   const int len = s.len;
   const Span span = span_of(len, s.row_rank, a.row_ranks);
   const int first = span.begin + s.ty, end = s.live ? span.end : 0;
-  const int frames = first < end ? (int)((unsigned)(end - first + s.rows - 1) / (unsigned)s.rows) : 0, kept = min(frames, a.kept);
+  const int kept = first < end ? (int)((unsigned)(end - first + s.rows - 1) / (unsigned)s.rows) : 0;
   const T *x = a.x.p + s.n * a.x.sn + first * a.x.st + s.c;
   const long long jump = s.rows * a.x.st;
   T *mine = reinterpret_cast<T *>(shared_raw) + threadIdx.x * V;  // frame i at mine + i * kThreads * V
@@ -264,18 +258,19 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_kernel(const NormArgs
     shift[v] = a.bias != nullptr && s.live ? a.bias[s.c + v] : A(0);
   }
   Moments<A> m;
-  if (frames > kept) add_frames<T, V>(m, frames - kept, [&](int i) { return load_raw<T, V>(x + (kept + i) * jump); });
   copies_done();
-  add_frames<T, V>(m, kept, [&](int i) { return load_shared<T, V>(mine + i * (kThreads * V)); });
+  constexpr int kBatch = 16;
+  for (int i0 = 0; i0 < kept; i0 += kBatch)
+    add_batch<T, V, kBatch>(m, min(kBatch, kept - i0), [&](int i) { return load_shared<T, V>(mine + (i0 + i) * (kThreads * V)); });
 
   // the block's: sum of the values, then of the squared deviations from their mean
   A count = A(span.end - span.begin) * A(s.some ? s.cols * V : 0);
   A total[1] = {m.count * m.mean};
-  team_sum(total, s, a.team, &slots[0]);
+  team_sum(total, s.team_id, a.team, &slots[0]);
   A mean = count > A(0) ? total[0] / count : A(0);
   const A d = m.mean - mean;
   A squares[1] = {m.m2 + m.count * d * d};
-  team_sum(squares, s, a.team, &slots[1]);
+  team_sum(squares, s.team_id, a.team, &slots[1]);
   A m2 = squares[0];
   if (s.size > 1) {
     auto cluster = cooperative_groups::this_cluster();
@@ -307,30 +302,12 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_kernel(const NormArgs
     };
 #pragma unroll 4
     for (int i = 0; i < kept; ++i) result(load_shared<T, V>(mine + i * (kThreads * V)), i);
-#pragma unroll 4
-    for (int i = kept; i < frames; ++i) result(load_raw<T, V>(x + i * jump), i);
   });
 }
 
 // Backward: the same seats.  MANY: a block takes `per_block` utterances, all of whose frames fit, one after the other and
 // keeps each channel's P1, P2 over all of them, so that few sets of parameter sums are left to be added (none, where one
 // block has all utterances).
-// body(x, grad_y, i) for the frames i in [from, to), which are not in shared memory: four frames' loads at a time
-template <typename T, int V, typename F>
-__device__ __forceinline__ void again(const T *x, long long jump, const T *gy, long long jump_y, int from, int to, F &&body) {
-  constexpr int U = 4;
-  x += from * jump, gy += from * jump_y;
-  for (int i0 = from; i0 < to; i0 += U, x += U * jump, gy += U * jump_y) {
-    Raw<T, V> xq[U], yq[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (i0 + i < to) xq[i] = load_raw<T, V>(x + i * jump), yq[i] = load_raw<T, V>(gy + i * jump_y);
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (i0 + i < to) body(xq[i], yq[i], i0 + i);
-  }
-}
-
 template <typename T, int V, int MB, bool MANY>
 __global__ void __launch_bounds__(kThreads, MB) norm_fused_backward_kernel(const NormArgs<T> a) {
   using A = Acc<T>;
@@ -357,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_backward_kernel(const
     const int len = MANY ? live_frames(a.lens, n, a.frames) : s.len;
     const Span span = span_of(len, s.row_rank, a.row_ranks);
     const int first = span.begin + s.ty, end = s.live ? span.end : 0;
-    const int frames = first < end ? (int)((unsigned)(end - first + s.rows - 1) / (unsigned)s.rows) : 0, kept = min(frames, a.kept);
+    const int kept = first < end ? (int)((unsigned)(end - first + s.rows - 1) / (unsigned)s.rows) : 0;
     const T *x = a.x.p + n * a.x.sn + first * a.x.st + s.c, *gy = a.grad_y.p + n * a.grad_y.sn + first * a.grad_y.st + s.c;
     const long long jump = s.rows * a.x.st, jump_y = s.rows * a.grad_y.st, leap = s.rows * a.grad_x.st;
     const T *from = x, *from_y = gy;
@@ -378,8 +355,6 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_backward_kernel(const
           q1[v] += gz, q2[v] += gz * d;
         }
       };
-      if constexpr (!MANY)
-        again<T, V>(x, jump, gy, jump_y, kept, frames, [&](const Raw<T, V> &xq, const Raw<T, V> &yq, int) { add(xq, yq); });
       copies_done();
 #pragma unroll 2
       for (int i = 0; i < kept; ++i)
@@ -392,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_backward_kernel(const
       else p1[v] = q1[v], p2[v] = q2[v];
       sums[0] += weight[v] * q1[v], sums[1] += weight[v] * q2[v];
     }
-    team_sum(sums, s, a.team, slots[buffer]);
+    team_sum(sums, s.team_id, a.team, slots[buffer]);
     A s1 = sums[0], s2 = sums[1];
     if (s.size > 1) {
       auto cluster = cooperative_groups::this_cluster();
@@ -423,7 +398,6 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_backward_kernel(const
 #pragma unroll 2
       for (int i = 0; i < kept; ++i)
         result(load_shared<T, V>(mine + i * (kThreads * V)), load_shared<T, V>(mine_y + i * (kThreads * V)), i);
-      if constexpr (!MANY) again<T, V>(x, jump, gy, jump_y, kept, frames, result);
     });
   }
   if (a.grad_weight == nullptr && a.grad_bias == nullptr) return;
@@ -446,238 +420,235 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_backward_kernel(const
   }
 }
 
-// ---- any size: pass over the tensor for the sums, pass again to normalise ------------------------------------------
+// ---- large groups: sums and result in two launches ---------------------------------------------------------------------
+//
+// Groups that a cluster's shared memory does not hold.  A block has `tx` packs of channels of one group and `chunk_rows`
+// of its utterance's frames; `slabs` blocks side by side have a frame of the group, `chunks` one after the other its
+// frames.  The first launch writes every block's sums; in the second, which is scheduled while the first drains, every
+// block adds its group's and normalises its part, read from L2 as a rule.  4 x 16384 x 256 channels, 8 groups, SiLU,
+// bfloat16: 27 us forward and 44 us backward (bytes alone: 10 and 15); 12 x 548..2191 x 549 float32, one group: 41 and 57
+// (12 and 22).
 
-struct ChunkSpan {
-  long long n, begin, end;  // frames of utterance n this block has
-  int k, c;                 // chunk, first channel of the thread
+// frames of a thread fetched together: 8, or 4 where two tensors of 16 bytes a thread would fill the registers (four with
+// the next four in flight were slower, 27 / 53 us below)
+template <int BYTES, bool BOTH>
+constexpr int kSpreadRows = BOTH && BYTES >= 16 ? 4 : 8;
+
+struct Part {  // a block's part of a group, and a thread's place in it
+  int n, len, g, c, ty, begin, end, entry, cols;
+  bool live;
 };
 template <typename T, int V>
-__device__ __forceinline__ ChunkSpan chunk_span(const NormArgs<T> &a, long long upto) {
-  long long b = blockIdx.x;
-  ChunkSpan s;
-  const int slab = (int)(b % a.slabs);
-  b /= a.slabs;
-  s.k = (int)(b % a.chunks), s.n = b / a.chunks;
-  const long long rows = ((long long)a.frames + a.chunks - 1) / a.chunks;
-  s.begin = s.k * rows;
-  s.end = s.begin + rows < upto ? s.begin + rows : upto;
-  s.c = (slab * a.tx + (int)(threadIdx.x % a.tx)) * V;
+__device__ __forceinline__ Part part_of(const NormArgs<T> &a) {
+  Part s;
+  s.n = (int)(blockIdx.z * 65535u + blockIdx.y);
+  s.len = s.n < a.batch ? live_frames(a.lens, s.n, a.frames) : 0;
+  const unsigned across = (unsigned)(a.groups * a.slabs), chunk = blockIdx.x / across, rest = blockIdx.x - chunk * across;
+  s.g = (int)(rest / (unsigned)a.slabs);
+  const int slab = (int)rest - s.g * a.slabs, left = a.packs - slab * a.tx;
+  s.cols = left < a.tx ? left : a.tx;
+  s.ty = (int)(threadIdx.x * a.packs_magic >> 20);  // threadIdx.x / tx
+  const int tx = (int)threadIdx.x - s.ty * a.tx;
+  s.live = s.ty < a.rows && tx < s.cols;
+  s.c = (s.g * a.packs + slab * a.tx + tx) * V;
+  s.begin = (int)chunk * a.chunk_rows;
+  s.end = s.begin + a.chunk_rows;  // of the frames there are room for; those of the utterance end at len
+  s.entry = (int)chunk * a.slabs + slab;
   return s;
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) norm_moments_kernel(const NormArgs<T> a) {
-  using A = Acc<T>;
-  __shared__ A mean_s[kThreads][V], m2_s[kThreads][V], count_s[kThreads];
-  const long long upto = live_frames(a.lens, blockIdx.x / ((long long)a.slabs * a.chunks), a.frames);
-  const ChunkSpan s = chunk_span<T, V>(a, upto);
-  const int ty = threadIdx.x / a.tx, rows = kThreads / a.tx;
-  A mean[V], m2[V], count = 0;
+// A thread's frames first, first + step, ... below `end`, U at a time: body(x, grad_y, frame, n) with n frames in x (and,
+// BOTH, in grad_y)
+template <typename T, int V, bool BOTH, int U, typename F>
+__device__ __forceinline__ void walk(const Frames<const T> &xf, const Frames<const T> &yf, int n, int c, int first, int step,
+                                     int end, F &&body) {
+  const T *x = xf.p + n * xf.sn + c, *gy = yf.p + n * yf.sn + c;
+  for (int t = first; t < end; t += U * step) {
+    Raw<T, V> xq[U], yq[BOTH ? U : 1];
 #pragma unroll
-  for (int v = 0; v < V; ++v) mean[v] = m2[v] = 0;
-  if (s.c < a.channels) {
-    for (long long t = s.begin + ty; t < s.end; t += rows) {
-      const Raw<T, V> p = load_raw<T, V>(a.x.p + s.n * a.x.sn + t * a.x.st + s.c);
-      count += A(1);
-      const A inv = A(1) / count;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const A value = element(p, v), delta = value - mean[v];
-        mean[v] += delta * inv;
-        m2[v] += delta * (value - mean[v]);
+    for (int i = 0; i < U; ++i)
+      if (t + i * step < end) {
+        xq[i] = load_raw<T, V>(x + (t + i * step) * xf.st);
+        if constexpr (BOTH) yq[i] = load_raw<T, V>(gy + (t + i * step) * yf.st);
       }
-    }
-  }
-#pragma unroll
-  for (int v = 0; v < V; ++v) mean_s[threadIdx.x][v] = mean[v], m2_s[threadIdx.x][v] = m2[v];
-  count_s[threadIdx.x] = count;
-  __syncthreads();
-  if (ty == 0 && s.c < a.channels) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      A total = count;
-      for (int r = 1; r < rows; ++r) {
-        const int o = r * a.tx + threadIdx.x;
-        join(mean[v], m2[v], total, mean_s[o][v], m2_s[o][v], count_s[o]);
-      }
-      A *out = a.part + (((long long)s.n * a.chunks + s.k) * a.channels + s.c + v) * 2;
-      out[0] = mean[v], out[1] = m2[v];
-    }
+    body(xq, yq, t, min(U, (int)((unsigned)(end - t + step - 1) / (unsigned)step)));
   }
 }
 
-// mean and rstd of one (utterance, group) from the chunks' moments
-template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_stats_kernel(const NormArgs<T> a) {
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads, 2) norm_moments_kernel(const NormArgs<T> a) {
   using A = Acc<T>;
-  __shared__ A mean_s[kThreads], m2_s[kThreads], count_s[kThreads];
-  const long long n = blockIdx.x / a.groups;
-  const int g = (int)(blockIdx.x % a.groups), per = a.channels / a.groups;
-  const long long upto = live_frames(a.lens, n, a.frames), rows = ((long long)a.frames + a.chunks - 1) / a.chunks;
-  A mean = 0, m2 = 0, count = 0;
-  for (long long i = threadIdx.x; i < (long long)a.chunks * per; i += kThreads) {
-    const long long k = i / per, begin = k * rows, end = begin + rows < upto ? begin + rows : upto;
-    const A *in = a.part + ((n * a.chunks + k) * a.channels + (long long)g * per + i % per) * 2;
-    if (end > begin) join(mean, m2, count, in[0], in[1], A(end - begin));
-  }
-  mean_s[threadIdx.x] = mean, m2_s[threadIdx.x] = m2, count_s[threadIdx.x] = count;
-  __syncthreads();
-  for (int half = kThreads / 2; half > 0; half >>= 1) {
-    if (threadIdx.x < half) {
-      join(mean, m2, count, mean_s[threadIdx.x + half], m2_s[threadIdx.x + half], count_s[threadIdx.x + half]);
-      mean_s[threadIdx.x] = mean, m2_s[threadIdx.x] = m2, count_s[threadIdx.x] = count;
-    }
-    __syncthreads();
-  }
+  constexpr int U = kSpreadRows<Raw<T, V>::kBytes, false>;
+  __shared__ __align__(16) A slots[2][kThreads / 32];
+  const Part s = part_of<T, V>(a);
+  if (s.n >= a.batch) return;
+  const int end = min(s.end, s.len);
+  Moments<A> m;
+  walk<T, V, false, U>(a.x, a.grad_y, s.n, s.c, s.begin + s.ty, a.rows, s.live ? end : 0,
+                    [&](Raw<T, V> (&xq)[U], Raw<T, V> (&)[1], int, int n) {
+                      add_batch<T, V, U>(m, n, [&](int i) { return xq[i]; });
+                    });
+  const A count = A(max(end - s.begin, 0)) * A(s.cols * V);
+  A total[1] = {m.count * m.mean};
+  team_sum(total, 0, kThreads, &slots[0]);
+  const A mean = count > A(0) ? total[0] / count : A(0), d = m.mean - mean;
+  A squares[1] = {m.m2 + m.count * d * d};
+  team_sum(squares, 0, kThreads, &slots[1]);
   if (threadIdx.x == 0) {
-    a.stats_out[2 * (long long)blockIdx.x] = mean;
-    a.stats_out[2 * (long long)blockIdx.x + 1] = count > A(0) ? A(1) / sqrt(m2 / count + a.eps) : A(0);
-  }
-}
-
-// the statistics and parameters of a thread's V channels
-template <typename T, int V>
-struct ChannelParams {
-  Acc<T> mean[V], rstd[V], weight[V], bias[V];
-  __device__ __forceinline__ void load(const NormArgs<T> &a, long long n, int c) {
-    const int per = a.channels / a.groups;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const Acc<T> *st = a.stats + (n * a.groups + (c + v) / per) * 2;
-      mean[v] = st[0], rstd[v] = st[1];
-      weight[v] = a.weight != nullptr ? a.weight[c + v] : Acc<T>(1);
-      bias[v] = a.bias != nullptr ? a.bias[c + v] : Acc<T>(0);
-    }
-  }
-};
-
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) norm_apply_kernel(const NormArgs<T> a) {
-  using A = Acc<T>;
-  const ChunkSpan s = chunk_span<T, V>(a, a.frames);
-  if (s.c >= a.channels) return;
-  const long long upto = live_frames(a.lens, s.n, a.frames);
-  ChannelParams<T, V> q;
-  q.load(a, s.n, s.c);
-  for (long long t = s.begin + threadIdx.x / a.tx; t < s.end; t += kThreads / a.tx) {
-    A o[V];
-    if (t < upto) {
-      const Raw<T, V> p = load_raw<T, V>(a.x.p + s.n * a.x.sn + t * a.x.st + s.c);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const A xhat = (element(p, v) - q.mean[v]) * q.rstd[v];
-        o[v] = act_value(xhat * q.weight[v] + q.bias[v], a.act);
-      }
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) o[v] = A(0);
-    }
-    store_raw<T, V>(a.y.p + s.n * a.y.sn + t * a.y.st + s.c, rounded<T, V>(o));
+    A *to = a.part + (((long long)s.n * a.groups + s.g) * a.entries + s.entry) * 3;
+    to[0] = mean, to[1] = squares[0], to[2] = count;
   }
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) norm_sums_kernel(const NormArgs<T> a) {
+__global__ void __launch_bounds__(kThreads, 2) norm_apply_kernel(const NormArgs<T> a) {
   using A = Acc<T>;
-  __shared__ A sum_s[kThreads][2 * V];
-  const long long upto = live_frames(a.lens, blockIdx.x / ((long long)a.slabs * a.chunks), a.frames);
-  const ChunkSpan s = chunk_span<T, V>(a, upto);
-  const int ty = threadIdx.x / a.tx, rows = kThreads / a.tx;
-  A sum[2 * V];
-#pragma unroll
-  for (int v = 0; v < 2 * V; ++v) sum[v] = 0;
-  if (s.c < a.channels) {
-    ChannelParams<T, V> q;
-    q.load(a, s.n, s.c);
-    for (long long t = s.begin + ty; t < s.end; t += rows) {
-      const Raw<T, V> p = load_raw<T, V>(a.x.p + s.n * a.x.sn + t * a.x.st + s.c);
-      const Raw<T, V> gy = load_raw<T, V>(a.grad_y.p + s.n * a.grad_y.sn + t * a.grad_y.st + s.c);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const A xhat = (element(p, v) - q.mean[v]) * q.rstd[v];
-        const A gz = element(gy, v) * act_slope(xhat * q.weight[v] + q.bias[v], a.act);
-        sum[2 * v] += gz, sum[2 * v + 1] += gz * xhat;
-      }
-    }
-  }
-#pragma unroll
-  for (int v = 0; v < 2 * V; ++v) sum_s[threadIdx.x][v] = sum[v];
-  __syncthreads();
-  if (ty == 0 && s.c < a.channels) {
-    A *out = a.part + (((long long)s.n * a.chunks + s.k) * a.channels + s.c) * 2;
-#pragma unroll
-    for (int v = 0; v < 2 * V; ++v) {
-      for (int r = 1; r < rows; ++r) sum[v] += sum_s[r * a.tx + threadIdx.x][v];
-      out[v] = sum[v];
-    }
-  }
-}
-
-// P1, P2 of every channel of one (utterance, group), and the group's two weighted sums over M
-template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_group_sums_kernel(const NormArgs<T> a) {
-  using A = Acc<T>;
-  __shared__ A s1[kThreads], s2[kThreads];
-  const long long n = blockIdx.x / a.groups;
-  const int g = (int)(blockIdx.x % a.groups), per = a.channels / a.groups;
-  A w1 = 0, w2 = 0;
-  for (int j = threadIdx.x; j < per; j += kThreads) {
-    const int c = g * per + j;
-    A p1 = 0, p2 = 0;
-    for (int k = 0; k < a.chunks; ++k) {
-      const A *in = a.part + ((n * a.chunks + k) * a.channels + c) * 2;
-      p1 += in[0], p2 += in[1];
-    }
-    a.sums[(n * a.channels + c) * 2] = p1, a.sums[(n * a.channels + c) * 2 + 1] = p2;
-    const A w = a.weight != nullptr ? a.weight[c] : A(1);
-    w1 += w * p1, w2 += w * p2;
-  }
-  s1[threadIdx.x] = w1, s2[threadIdx.x] = w2;
-  __syncthreads();
-  for (int half = kThreads / 2; half > 0; half >>= 1) {
-    if (threadIdx.x < half) s1[threadIdx.x] += s1[threadIdx.x + half], s2[threadIdx.x] += s2[threadIdx.x + half];
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) {
-    const A count = A(live_frames(a.lens, n, a.frames)) * A(per);
-    a.gsums[2 * (long long)blockIdx.x] = count > A(0) ? s1[0] / count : A(0);
-    a.gsums[2 * (long long)blockIdx.x + 1] = count > A(0) ? s2[0] / count : A(0);
-  }
-}
-
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) norm_grad_input_kernel(const NormArgs<T> a) {
-  using A = Acc<T>;
-  const ChunkSpan s = chunk_span<T, V>(a, a.frames);
-  if (s.c >= a.channels) return;
-  const long long upto = live_frames(a.lens, s.n, a.frames);
-  const int per = a.channels / a.groups;
-  ChannelParams<T, V> q;
-  q.load(a, s.n, s.c);
-  A s1[V], s2[V];
+  constexpr int U = kSpreadRows<Raw<T, V>::kBytes, false>;
+  __shared__ __align__(16) A slots[3][kThreads / 32];
+  const Part s = part_of<T, V>(a);
+  const int end = min(s.end, s.len), first = s.begin + s.ty, step = a.rows;
+  A scale[V], shift[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const A *in = a.gsums + (s.n * a.groups + (s.c + v) / per) * 2;
-    s1[v] = in[0], s2[v] = in[1];
+    scale[v] = a.weight != nullptr && s.live ? a.weight[s.c + v] : A(1);
+    shift[v] = a.bias != nullptr && s.live ? a.bias[s.c + v] : A(0);
   }
-  for (long long t = s.begin + threadIdx.x / a.tx; t < s.end; t += kThreads / a.tx) {
-    A o[V];
-    if (t < upto) {
-      const Raw<T, V> p = load_raw<T, V>(a.x.p + s.n * a.x.sn + t * a.x.st + s.c);
-      const Raw<T, V> gy = load_raw<T, V>(a.grad_y.p + s.n * a.grad_y.sn + t * a.grad_y.st + s.c);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const A xhat = (element(p, v) - q.mean[v]) * q.rstd[v];
-        const A gz = element(gy, v) * act_slope(xhat * q.weight[v] + q.bias[v], a.act);
-        o[v] = q.rstd[v] * (gz * q.weight[v] - s1[v] - xhat * s2[v]);
-      }
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) o[v] = A(0);
-    }
-    store_raw<T, V>(a.grad_x.p + s.n * a.grad_x.sn + t * a.grad_x.st + s.c, rounded<T, V>(o));
+  tc::grid_dependency_wait();  // the sums
+  if (s.n >= a.batch) return;
+  const A *in = a.part + ((long long)s.n * a.groups + s.g) * a.entries * 3;
+  A sums[2] = {A(0), A(0)}, squares[1] = {A(0)};
+  for (int e = threadIdx.x; e < a.entries; e += kThreads) sums[0] += in[3 * e + 2], sums[1] += in[3 * e + 2] * in[3 * e];
+  team_sum(sums, 0, kThreads, &slots[0]);
+  const A count = sums[0], mean = count > A(0) ? sums[1] / count : A(0);
+  for (int e = threadIdx.x; e < a.entries; e += kThreads) {
+    const A d = in[3 * e] - mean;
+    squares[0] += in[3 * e + 1] + in[3 * e + 2] * d * d;
   }
+  team_sum(squares, 0, kThreads, &slots[2]);
+  const A rstd = count > A(0) ? A(1) / sqrt(squares[0] / count + a.eps) : A(0);
+  if (a.stats_out != nullptr && s.entry == 0 && threadIdx.x == 0) {
+    A *out = a.stats_out + ((long long)s.n * a.groups + s.g) * 2;
+    out[0] = mean, out[1] = rstd;
+  }
+  if (!s.live) return;
+#pragma unroll
+  for (int v = 0; v < V; ++v) scale[v] *= rstd;
+  T *y = a.y.p + s.n * a.y.sn + s.c;
+  by_act(a.act, [&](auto act) {
+    walk<T, V, false, U>(a.x, a.grad_y, s.n, s.c, first, step, end,
+                      [&](Raw<T, V> (&xq)[U], Raw<T, V> (&)[1], int t, int n) {
+#pragma unroll
+                        for (int i = 0; i < U; ++i) {
+                          if (i < n) {
+                            A o[V];
+#pragma unroll
+                            for (int v = 0; v < V; ++v)
+                              o[v] = act_value((element(xq[i], v) - mean) * scale[v] + shift[v], decltype(act)::value);
+                            store_raw<T, V>(y + (t + i * step) * a.y.st, rounded<T, V>(o));
+                          }
+                        }
+                      });
+  });
+  const int room = min(s.end, a.frames), from = max(s.len - s.begin, 0);  // frames behind the utterance's end
+  clear_from<T, V>(a.y, s.n, s.c, first + (from > s.ty ? (from - s.ty + step - 1) / step * step : 0), step, room);
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads, 2) norm_sums_kernel(const NormArgs<T> a) {
+  using A = Acc<T>;
+  constexpr int U = kSpreadRows<Raw<T, V>::kBytes, true>;
+  __shared__ __align__(16) A slots[2][kThreads / 32];
+  __shared__ A columns[2 * V][kThreads];
+  const Part s = part_of<T, V>(a);
+  if (s.n >= a.batch) return;
+  const int end = s.live ? min(s.end, s.len) : 0, first = s.begin + s.ty;
+  const A *st = a.stats + ((long long)s.n * a.groups + s.g) * 2, mean = st[0], rstd = st[1];
+  A scale[V], weight[V], bias[V], q1[V], q2[V], sums[2] = {A(0), A(0)};
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    weight[v] = a.weight != nullptr && s.live ? a.weight[s.c + v] : A(1);
+    bias[v] = a.bias != nullptr && s.live ? a.bias[s.c + v] : A(0);
+    q1[v] = q2[v] = 0, scale[v] = rstd * weight[v];
+  }
+  by_act(a.act, [&](auto act) {
+    walk<T, V, true, U>(a.x, a.grad_y, s.n, s.c, first, a.rows, end,
+                     [&](Raw<T, V> (&xq)[U], Raw<T, V> (&yq)[U], int, int n) {
+#pragma unroll
+                       for (int i = 0; i < U; ++i)
+                         if (i < n)
+#pragma unroll
+                           for (int v = 0; v < V; ++v) {
+                             const A d = element(xq[i], v) - mean;
+                             const A gz = element(yq[i], v) * act_slope(d * scale[v] + bias[v], decltype(act)::value);
+                             q1[v] += gz, q2[v] += gz * d;
+                           }
+                     });
+  });
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    q2[v] *= rstd;
+    sums[0] += weight[v] * q1[v], sums[1] += weight[v] * q2[v];
+    columns[2 * v][threadIdx.x] = q1[v], columns[2 * v + 1][threadIdx.x] = q2[v];
+  }
+  team_sum(sums, 0, kThreads, slots);  // its barrier is the columns' too
+  if (threadIdx.x == 0) {
+    A *to = a.gsums + (((long long)s.n * a.groups + s.g) * a.entries + s.entry) * 2;
+    to[0] = sums[0], to[1] = sums[1];
+  }
+  const int chunk = s.entry / a.slabs, first_pack = s.g * a.packs + (s.entry - chunk * a.slabs) * a.tx;
+  A *to = a.part + ((long long)s.n * a.chunks + chunk) * a.channels * 2;
+  for (int q = threadIdx.x; q < 2 * V * s.cols; q += kThreads) {
+    const int v = q / s.cols, tx = q - v * s.cols;
+    A sum = 0;
+#pragma unroll 8
+    for (int r = 0; r < a.rows; ++r) sum += columns[v][r * a.tx + tx];
+    to[((first_pack + tx) * V + v / 2) * 2 + v % 2] = sum;
+  }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads, 2) norm_grad_input_kernel(const NormArgs<T> a) {
+  using A = Acc<T>;
+  constexpr int U = kSpreadRows<Raw<T, V>::kBytes, true>;
+  __shared__ __align__(16) A slots[2][kThreads / 32];
+  const Part s = part_of<T, V>(a);
+  if (s.n >= a.batch) return;
+  const int end = s.live ? min(s.end, s.len) : 0, first = s.begin + s.ty;
+  const A *st = a.stats + ((long long)s.n * a.groups + s.g) * 2, mean = st[0], rstd = st[1];
+  A scale[V], bias[V], sums[2] = {A(0), A(0)};
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    scale[v] = rstd * (a.weight != nullptr && s.live ? a.weight[s.c + v] : A(1));
+    bias[v] = a.bias != nullptr && s.live ? a.bias[s.c + v] : A(0);
+  }
+  tc::grid_dependency_wait();  // the sums
+  const A *in = a.gsums + ((long long)s.n * a.groups + s.g) * a.entries * 2;
+  for (int e = threadIdx.x; e < a.entries; e += kThreads) sums[0] += in[2 * e], sums[1] += in[2 * e + 1];
+  team_sum(sums, 0, kThreads, slots);
+  const A count = A(s.len) * A(a.channels / a.groups), inv = count > A(0) ? A(1) / count : A(0);
+  const A s1 = sums[0] * inv * rstd, s2 = sums[1] * inv * rstd * rstd;  // gx = scale gz - s1 - (x - mean) s2
+  if (!s.live) return;
+  T *gx = a.grad_x.p + s.n * a.grad_x.sn + s.c;
+  by_act(a.act, [&](auto act) {
+    walk<T, V, true, U>(a.x, a.grad_y, s.n, s.c, first, a.rows, end,
+                     [&](Raw<T, V> (&xq)[U], Raw<T, V> (&yq)[U], int t, int n) {
+#pragma unroll
+                       for (int i = 0; i < U; ++i) {
+                         if (i < n) {
+                           A o[V];
+#pragma unroll
+                           for (int v = 0; v < V; ++v) {
+                             const A d = element(xq[i], v) - mean;
+                             const A gz = element(yq[i], v) * act_slope(d * scale[v] + bias[v], decltype(act)::value);
+                             o[v] = gz * scale[v] - (d * s2 + s1);
+                           }
+                           store_raw<T, V>(gx + (t + i * a.rows) * a.grad_x.st, rounded<T, V>(o));
+                         }
+                       }
+                     });
+  });
+  const int room = min(s.end, a.frames), from = max(s.len - s.begin, 0), step = a.rows;
+  clear_from<T, V>(a.grad_x, s.n, s.c, first + (from > s.ty ? (from - s.ty + step - 1) / step * step : 0), step, room);
 }
 
 // gweight and gbias: P2 and P1 of `parts` sets added; a block has 32 channels, 8 threads each, whose sums are joined in
@@ -712,13 +683,6 @@ __global__ void __launch_bounds__(kThreads) norm_grad_params_kernel(const NormAr
 // against 39, and so would backward)
 constexpr int kept_bytes(int tensors, size_t element) { return (tensors == 1 && element == 2 ? 72 : 108) * 1024; }
 
-int chunks_for(int64_t batch, int64_t frames, int64_t channels) {
-  // enough blocks to fill the device a few times over, at least 32 frames in each
-  const int64_t slabs = (channels + 31) / 32;
-  const int64_t want = (148 * 16 + batch * slabs - 1) / std::max<int64_t>(batch * slabs, 1);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, (frames + 31) / 32, (int64_t)kMaxChunks}));
-}
-
 // Elements a thread moves at once: a power of two that divides a group's channels, so that they share its statistics
 template <typename T>
 int vector_width(const NormArgs<T> &a) {
@@ -731,7 +695,7 @@ int vector_width(const NormArgs<T> &a) {
 }
 
 struct FusedPlan {
-  bool use = false, fits = false;  // every frame is kept
+  bool use = false;  // a cluster holds a group
   int team = 0, col_ranks = 1, row_ranks = 1, kept = 0;
   long long blocks_per_utterance = 0;
 };
@@ -748,45 +712,54 @@ FusedPlan plan_fused(int64_t batch, int64_t frames, int64_t groups, int64_t per,
   const int64_t rows = std::max<int64_t>(1, p.team / packs);
   auto kept = [&] { return ((frames + p.row_ranks - 1) / p.row_ranks + rows - 1) / rows; };
   while (p.team == kThreads && p.col_ranks * p.row_ranks < kMaxRanks && kept() > most) p.row_ranks *= 2;
-  p.kept = (int)std::min<int64_t>(kept(), most), p.fits = kept() <= most;
+  p.kept = (int)std::min<int64_t>(kept(), most);
   const int teams = kThreads / p.team;
   p.blocks_per_utterance = (groups + teams - 1) / teams * p.col_ranks * p.row_ranks;
-  // a few groups far larger than a cluster's registers: too few blocks to reach the memory's rate
-  p.use = kept() <= 2 * most || batch * p.blocks_per_utterance >= 128;
+  p.use = kept() <= most;
   return p;
 }
 
-// Whether some alignment of the tensors leaves the shape to the kernels that pass over it twice
-bool may_pass_twice(int64_t batch, int64_t frames, int64_t groups, int64_t per, size_t element) {
-  for (int V : {1, 2, 4, 8})
-    if (per % V == 0 && !(plan_fused(batch, frames, groups, per, V, 1, element).use &&
-                          plan_fused(batch, frames, groups, per, V, 2, element).use))
-      return true;
-  return false;
+// The division of groups that do not fit: up to 64 packs a block and 32 frames a thread (16: 27 and 48 us at the shape above,
+// 64: 29 and 52), at most about 1024 parts of a group
+struct SpreadPlan {
+  int tx, slabs, rows, chunks, chunk_rows;
+};
+SpreadPlan plan_spread(int64_t frames, int64_t per, int V) {
+  SpreadPlan p;
+  const int64_t packs = per / V;
+  p.slabs = (int)((packs + 63) / 64), p.tx = (int)((packs + p.slabs - 1) / p.slabs), p.rows = kThreads / p.tx;
+  const int64_t most = std::max<int64_t>(1, 1024 / p.slabs), each = (int64_t)p.rows * 32;
+  const int64_t want = std::max<int64_t>(1, std::min((frames + each - 1) / each, most));
+  p.chunk_rows = (int)((frames + want - 1) / want);
+  p.chunks = p.chunk_rows > 0 ? (int)((frames + p.chunk_rows - 1) / p.chunk_rows) : 1;
+  return p;
 }
 
 // Utterances a backward block takes: all of them where that is little (one launch less), one where that leaves few sets
 // of parameter sums, else as many as leave about three rounds of two blocks a multiprocessor
 int64_t utterances_a_block(int64_t batch, int64_t frames, int64_t channels, const FusedPlan &p, size_t element) {
-  if (!p.fits) return 1;
   if (batch <= 8 && (size_t)(frames * channels) * element <= (512u << 10)) return batch;
   if (batch * p.row_ranks <= 512) return 1;
   return std::max<int64_t>(1, batch * p.blocks_per_utterance / (148 * 6));
 }
 
-// workspace in elements of the accumulation type.  The fused kernels need the sets of parameter sums, backward; the others (batch, chunks, channels, 2), (batch, channels, 2) and (batch, groups, 2).
+// Workspace in elements of the accumulation type, for whichever width the tensors' alignment allows
 size_t workspace_elements(int64_t batch, int64_t frames, int64_t channels, int64_t groups, size_t element, bool backward) {
   if (batch <= 0 || frames < 0 || channels <= 0 || groups <= 0 || channels % groups != 0) return 0;
+  const int64_t per = channels / groups;
   size_t need = 0;
-  for (int V : {1, 2, 4, 8}) {
-    if (!backward || channels / groups % V != 0) continue;
-    const FusedPlan p = plan_fused(batch, frames, groups, channels / groups, V, 2, element);
-    if (!p.use) continue;
-    const int64_t each = utterances_a_block(batch, frames, channels, p, element);
-    need = std::max(need, (size_t)((batch + each - 1) / each) * p.row_ranks * (size_t)channels * 2);
+  for (int V : {1, 2, 16 / (int)element}) {
+    if (per % V != 0) continue;
+    const FusedPlan p = plan_fused(batch, frames, groups, per, V, backward ? 2 : 1, element);
+    if (p.use) {  // sets of parameter sums
+      const int64_t each = utterances_a_block(batch, frames, channels, p, element);
+      if (backward) need = std::max(need, (size_t)((batch + each - 1) / each) * p.row_ranks * (size_t)channels * 2);
+    } else {
+      const SpreadPlan q = plan_spread(frames, per, V);
+      const size_t entries = (size_t)batch * groups * q.chunks * q.slabs;
+      need = std::max(need, backward ? (size_t)batch * q.chunks * channels * 2 + entries * 2 : entries * 3);
+    }
   }
-  if (may_pass_twice(batch, frames, groups, channels / groups, element))
-    need = std::max(need, (size_t)batch * (size_t)channels * 2 * ((size_t)chunks_for(batch, frames, channels) + 2));
   return need;
 }
 
@@ -811,23 +784,18 @@ int prepare(const char *who, NormArgs<T> &a, int64_t batch, int64_t frames, int6
 }
 
 template <typename T>
-void prepare_twice(NormArgs<T> &a) {
-  a.chunks = chunks_for(a.batch, a.frames, a.channels);
-  a.sums = a.part + (size_t)a.batch * a.chunks * a.channels * 2;
-  a.gsums = a.sums + (size_t)a.batch * a.channels * 2;
-}
-
-template <typename T>
-long long grid_for(NormArgs<T> &a, int V) {
-  int tx = 1;
-  while (tx < 32 && tx * V < a.channels) tx *= 2;
-  a.tx = tx, a.slabs = (a.channels + tx * V - 1) / (tx * V);
-  return (long long)a.batch * a.chunks * a.slabs;
+SpreadPlan take_spread(NormArgs<T> &a, int V) {
+  const SpreadPlan p = plan_spread(a.frames, a.channels / a.groups, V);
+  a.packs = a.channels / a.groups / V;
+  a.tx = p.tx, a.slabs = p.slabs, a.rows = p.rows, a.chunks = p.chunks, a.chunk_rows = p.chunk_rows;
+  a.entries = p.chunks * p.slabs, a.packs_magic = ((1u << 20) + p.tx - 1) / p.tx;
+  a.gsums = a.part + (size_t)a.batch * a.chunks * a.channels * 2;
+  return p;
 }
 
 template <typename K, typename T>
 int launch(const char *who, K kernel, const NormArgs<T> &a, long long blocks, int cluster, size_t shared, cudaStream_t st,
-           long long utterances = 1) {
+           long long utterances, bool after_predecessor = false) {
   if (blocks > 0x7fffffffLL) return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many blocks");
   cudaLaunchConfig_t cfg = {};
   const unsigned planes = (unsigned)((utterances + 65534) / 65535);  // the grid's second extent ends at 65535
@@ -839,9 +807,16 @@ int launch(const char *who, K kernel, const NormArgs<T> &a, long long blocks, in
     if (err != cudaSuccess) return fail(MELLIN_ERR_LAUNCH, std::string(who) + ": " + cudaGetErrorString(err));
   }
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr, cfg.numAttrs = cluster > 1 ? 1 : 0;
+  cfg.attrs = attr;
+  if (cluster > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  } else if (after_predecessor && dependent_launch_enabled()) {  // the kernel waits for the one before it by itself
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+  }
   const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, a);
   if (err != cudaSuccess) return fail(MELLIN_ERR_LAUNCH, std::string(who) + ": " + cudaGetErrorString(err));
   return launched(who);
@@ -897,13 +872,11 @@ int run_forward(NormArgs<T> a, int64_t batch, int64_t frames, int64_t channels, 
       constexpr int V = decltype(width)::value;
       const FusedPlan p = plan_fused(batch, frames, groups, channels / groups, V, 1, sizeof(T));
       if (p.use) return launch_fused<T, V, sizeof(T) == 2 ? 3 : 2>(who, a, p, st);
-      prepare_twice(a);
-      if (a.stats_out == nullptr) a.stats_out = a.gsums;
-      a.stats = a.stats_out;
-      const long long blocks = grid_for(a, V);
-      if ((rc = launch(who, norm_moments_kernel<T, V>, a, blocks, 1, 0, st)) != MELLIN_OK) return rc;
-      if ((rc = launch(who, norm_stats_kernel<T>, a, batch * groups, 1, 0, st)) != MELLIN_OK) return rc;
-      return launch(who, norm_apply_kernel<T, V>, a, blocks, 1, 0, st);
+      if (frames == 0) return MELLIN_OK;  // no statistics either: backward does not look at them
+      const SpreadPlan q = take_spread(a, V);
+      const long long blocks = groups * q.slabs * q.chunks;
+      if ((rc = launch(who, norm_moments_kernel<T, V>, a, blocks, 1, 0, st, batch)) != MELLIN_OK) return rc;
+      return launch(who, norm_apply_kernel<T, V>, a, blocks, 1, 0, st, batch, true);
     });
   });
 }
@@ -929,14 +902,16 @@ int run_backward(NormArgs<T> a, int64_t batch, int64_t frames, int64_t channels,
           parts = a.parts, sums = a.part;
           return rc;
         }
-        prepare_twice(a);
-        parts = (int)batch, sums = a.sums;
-        const long long blocks = grid_for(a, V);
-        if ((rc = launch(who, norm_sums_kernel<T, V>, a, blocks, 1, 0, st)) != MELLIN_OK) return rc;
-        if ((rc = launch(who, norm_group_sums_kernel<T>, a, batch * groups, 1, 0, st)) != MELLIN_OK) return rc;
-        rc = launch(who, norm_grad_input_kernel<T, V>, a, blocks, 1, 0, st);
-        a.parts = 0;  // the sums are still to be added, whatever their number
-        return rc;
+        if (frames == 0) {  // no sets of sums: zeros
+          parts = a.parts = 0;
+          return MELLIN_OK;
+        }
+        const SpreadPlan q = take_spread(a, V);
+        const long long blocks = groups * q.slabs * q.chunks, all = batch * q.chunks;
+        if (all > 0x7fffffffLL) return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many utterances times frames");
+        parts = (int)all, sums = a.part, a.parts = 0;  // the sums are still to be added, whatever their number
+        if ((rc = launch(who, norm_sums_kernel<T, V>, a, blocks, 1, 0, st, batch)) != MELLIN_OK) return rc;
+        return launch(who, norm_grad_input_kernel<T, V>, a, blocks, 1, 0, st, batch, true);
       });
       if (rc != MELLIN_OK || a.parts == 1) return rc;
     }
