@@ -420,13 +420,36 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_backward_kernel(const
   }
 }
 
+// gweight and gbias of 32 channels: P2 and P1 of the `parts` sets at a.part added, 8 threads a channel, whose sums are
+// joined in order.  All threads of a block call it.
+template <typename T>
+__device__ __forceinline__ void add_parts(const NormArgs<T> &a, int parts, int block) {
+  using A = Acc<T>;
+  __shared__ A s1[kThreads], s2[kThreads];
+  const int c = block * 32 + (int)(threadIdx.x & 31);
+  A p1 = 0, p2 = 0;
+  if (c < a.channels) {
+#pragma unroll 4
+    for (long long n = threadIdx.x >> 5; n < parts; n += kThreads / 32) {
+      const A *in = a.part + (n * a.channels + c) * 2;
+      p1 += in[0], p2 += in[1];
+    }
+  }
+  s1[threadIdx.x] = p1, s2[threadIdx.x] = p2;
+  __syncthreads();
+  if (threadIdx.x >= 32 || c >= a.channels) return;
+  for (int i = 1; i < kThreads / 32; ++i) p1 += s1[i * 32 + threadIdx.x], p2 += s2[i * 32 + threadIdx.x];
+  if (a.grad_weight != nullptr) a.grad_weight[c] = p2;
+  if (a.grad_bias != nullptr) a.grad_bias[c] = p1;
+}
+
 // ---- large groups: sums and result in two launches ---------------------------------------------------------------------
 //
 // Groups that a cluster's shared memory does not hold.  A block has `tx` packs of channels of one group and `chunk_rows`
 // of its utterance's frames; `slabs` blocks side by side have a frame of the group, `chunks` one after the other its
 // frames.  The first launch writes every block's sums; in the second, which is scheduled while the first drains, every
 // block adds its group's and normalises its part, read from L2 as a rule.  4 x 16384 x 256 channels, 8 groups, SiLU,
-// bfloat16: 27 us forward and 44 us backward (bytes alone: 10 and 15); 12 x 548..2191 x 549 float32, one group: 41 and 57
+// bfloat16: 25 us forward and 42 us backward (bytes alone: 10 and 15); 12 x 548..2191 x 549 float32, one group: 39 and 55
 // (12 and 22).
 
 // frames of a thread fetched together: 8, or 4 where two tensors of 16 bytes a thread would fill the registers (four with
@@ -476,7 +499,7 @@ __device__ __forceinline__ void walk(const Frames<const T> &xf, const Frames<con
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads, 2) norm_moments_kernel(const NormArgs<T> a) {
+__global__ void __launch_bounds__(kThreads, 3) norm_moments_kernel(const NormArgs<T> a) {
   using A = Acc<T>;
   constexpr int U = kSpreadRows<Raw<T, V>::kBytes, false>;
   __shared__ __align__(16) A slots[2][kThreads / 32];
@@ -501,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_moments_kernel(const NormArg
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads, 2) norm_apply_kernel(const NormArgs<T> a) {
+__global__ void __launch_bounds__(kThreads, 3) norm_apply_kernel(const NormArgs<T> a) {
   using A = Acc<T>;
   constexpr int U = kSpreadRows<Raw<T, V>::kBytes, false>;
   __shared__ __align__(16) A slots[3][kThreads / 32];
@@ -611,6 +634,13 @@ __global__ void __launch_bounds__(kThreads, 2) norm_grad_input_kernel(const Norm
   using A = Acc<T>;
   constexpr int U = kSpreadRows<Raw<T, V>::kBytes, true>;
   __shared__ __align__(16) A slots[2][kThreads / 32];
+  const int parts_of_all = a.groups * a.slabs * a.chunks;
+  if ((int)blockIdx.x >= parts_of_all) {  // the blocks behind the parts of the first utterance add the parameters' sums
+    if (blockIdx.y != 0 || blockIdx.z != 0) return;
+    tc::grid_dependency_wait();
+    add_parts(a, a.batch * a.chunks, (int)blockIdx.x - parts_of_all);
+    return;
+  }
   const Part s = part_of<T, V>(a);
   if (s.n >= a.batch) return;
   const int end = s.live ? min(s.end, s.len) : 0, first = s.begin + s.ty;
@@ -651,28 +681,10 @@ __global__ void __launch_bounds__(kThreads, 2) norm_grad_input_kernel(const Norm
   clear_from<T, V>(a.grad_x, s.n, s.c, first + (from > s.ty ? (from - s.ty + step - 1) / step * step : 0), step, room);
 }
 
-// gweight and gbias: P2 and P1 of `parts` sets added; a block has 32 channels, 8 threads each, whose sums are joined in
-// order
 template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_grad_params_kernel(const NormArgs<T> a, const Acc<T> *sums, int parts) {
-  using A = Acc<T>;
-  __shared__ A s1[kThreads], s2[kThreads];
-  const int c = blockIdx.x * 32 + (int)(threadIdx.x & 31);
-  A p1 = 0, p2 = 0;
+__global__ void __launch_bounds__(kThreads) norm_grad_params_kernel(const NormArgs<T> a, int parts) {
   tc::grid_dependency_wait();
-  if (c < a.channels) {
-#pragma unroll 4
-    for (long long n = threadIdx.x >> 5; n < parts; n += kThreads / 32) {
-      const A *in = sums + (n * a.channels + c) * 2;
-      p1 += in[0], p2 += in[1];
-    }
-  }
-  s1[threadIdx.x] = p1, s2[threadIdx.x] = p2;
-  __syncthreads();
-  if (threadIdx.x >= 32 || c >= a.channels) return;
-  for (int i = 1; i < kThreads / 32; ++i) p1 += s1[i * 32 + threadIdx.x], p2 += s2[i * 32 + threadIdx.x];
-  if (a.grad_weight != nullptr) a.grad_weight[c] = p2;
-  if (a.grad_bias != nullptr) a.grad_bias[c] = p1;
+  add_parts(a, parts, (int)blockIdx.x);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
@@ -715,21 +727,27 @@ FusedPlan plan_fused(int64_t batch, int64_t frames, int64_t groups, int64_t per,
   p.kept = (int)std::min<int64_t>(kept(), most);
   const int teams = kThreads / p.team;
   p.blocks_per_utterance = (groups + teams - 1) / teams * p.col_ranks * p.row_ranks;
-  p.use = kept() <= most;
+  // clusters of eight, which find few places at a time, lose to the two launches above about one round of them: 20 x 5000
+  // x 128, 4 groups, float32 33 us against 23 forward; 8 x 1200 x 512, 8 groups, backward 19 against 25
+  const bool many = p.col_ranks * p.row_ranks == kMaxRanks && (size_t)(batch * frames * groups * per) * element > (24u << 20);
+  p.use = kept() <= most && !many;
   return p;
 }
 
-// The division of groups that do not fit: up to 64 packs a block and 32 frames a thread (16: 27 and 48 us at the shape above,
-// 64: 29 and 52), at most about 1024 parts of a group
+// The division of groups that do not fit: up to 64 packs a block; as many chunks of frames as fill the multiprocessors
+// (three blocks each forward, two backward) a whole number of times (a last round of a few blocks costs as much as a full one), with 16 to about 64
+// frames a thread and at most about 1024 parts of a group
 struct SpreadPlan {
   int tx, slabs, rows, chunks, chunk_rows;
 };
-SpreadPlan plan_spread(int64_t frames, int64_t per, int V) {
+SpreadPlan plan_spread(int64_t batch, int64_t frames, int64_t groups, int64_t per, int V, bool backward) {
   SpreadPlan p;
   const int64_t packs = per / V;
   p.slabs = (int)((packs + 63) / 64), p.tx = (int)((packs + p.slabs - 1) / p.slabs), p.rows = kThreads / p.tx;
-  const int64_t most = std::max<int64_t>(1, 1024 / p.slabs), each = (int64_t)p.rows * 32;
-  const int64_t want = std::max<int64_t>(1, std::min((frames + each - 1) / each, most));
+  const int64_t base = batch * groups * p.slabs, slots = (backward ? 2 : 3) * 148, each = frames / p.rows;  // frames of a thread in all chunks
+  const int64_t rounds = std::max<int64_t>(1, (int64_t)((long double)each * base / (64 * slots) + 0.999L));
+  int64_t want = std::min(rounds * slots / std::max<int64_t>(base, 1), (each + 15) / 16);
+  want = std::max<int64_t>(1, std::min<int64_t>(want, std::max(1, 1024 / p.slabs)));
   p.chunk_rows = (int)((frames + want - 1) / want);
   p.chunks = p.chunk_rows > 0 ? (int)((frames + p.chunk_rows - 1) / p.chunk_rows) : 1;
   return p;
@@ -755,7 +773,7 @@ size_t workspace_elements(int64_t batch, int64_t frames, int64_t channels, int64
       const int64_t each = utterances_a_block(batch, frames, channels, p, element);
       if (backward) need = std::max(need, (size_t)((batch + each - 1) / each) * p.row_ranks * (size_t)channels * 2);
     } else {
-      const SpreadPlan q = plan_spread(frames, per, V);
+      const SpreadPlan q = plan_spread(batch, frames, groups, per, V, backward);
       const size_t entries = (size_t)batch * groups * q.chunks * q.slabs;
       need = std::max(need, backward ? (size_t)batch * q.chunks * channels * 2 + entries * 2 : entries * 3);
     }
@@ -784,8 +802,8 @@ int prepare(const char *who, NormArgs<T> &a, int64_t batch, int64_t frames, int6
 }
 
 template <typename T>
-SpreadPlan take_spread(NormArgs<T> &a, int V) {
-  const SpreadPlan p = plan_spread(a.frames, a.channels / a.groups, V);
+SpreadPlan take_spread(NormArgs<T> &a, int V, bool backward) {
+  const SpreadPlan p = plan_spread(a.batch, a.frames, a.groups, a.channels / a.groups, V, backward);
   a.packs = a.channels / a.groups / V;
   a.tx = p.tx, a.slabs = p.slabs, a.rows = p.rows, a.chunks = p.chunks, a.chunk_rows = p.chunk_rows;
   a.entries = p.chunks * p.slabs, a.packs_magic = ((1u << 20) + p.tx - 1) / p.tx;
@@ -873,7 +891,7 @@ int run_forward(NormArgs<T> a, int64_t batch, int64_t frames, int64_t channels, 
       const FusedPlan p = plan_fused(batch, frames, groups, channels / groups, V, 1, sizeof(T));
       if (p.use) return launch_fused<T, V, sizeof(T) == 2 ? 3 : 2>(who, a, p, st);
       if (frames == 0) return MELLIN_OK;  // no statistics either: backward does not look at them
-      const SpreadPlan q = take_spread(a, V);
+      const SpreadPlan q = take_spread(a, V, false);
       const long long blocks = groups * q.slabs * q.chunks;
       if ((rc = launch(who, norm_moments_kernel<T, V>, a, blocks, 1, 0, st, batch)) != MELLIN_OK) return rc;
       return launch(who, norm_apply_kernel<T, V>, a, blocks, 1, 0, st, batch, true);
@@ -889,7 +907,6 @@ int run_backward(NormArgs<T> a, int64_t batch, int64_t frames, int64_t channels,
     int rc = prepare(who, a, batch, frames, channels, groups, act, true, workspace, workspace_bytes);
     if (rc != MELLIN_OK || channels == 0) return rc;
     auto st = static_cast<cudaStream_t>(stream);
-    const Acc<T> *sums = nullptr;
     int parts = 0;
     if (batch > 0) {
       if (a.stats == nullptr || (frames > 0 && (a.x.p == nullptr || a.grad_y.p == nullptr || a.grad_x.p == nullptr)))
@@ -899,25 +916,26 @@ int run_backward(NormArgs<T> a, int64_t batch, int64_t frames, int64_t channels,
         const FusedPlan p = plan_fused(batch, frames, groups, channels / groups, V, 2, sizeof(T));
         if (p.use) {
           rc = launch_fused_backward<T, V, 2>(who, a, p, st);
-          parts = a.parts, sums = a.part;
+          parts = a.parts;
           return rc;
         }
         if (frames == 0) {  // no sets of sums: zeros
           parts = a.parts = 0;
           return MELLIN_OK;
         }
-        const SpreadPlan q = take_spread(a, V);
-        const long long blocks = groups * q.slabs * q.chunks, all = batch * q.chunks;
-        if (all > 0x7fffffffLL) return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many utterances times frames");
-        parts = (int)all, sums = a.part, a.parts = 0;  // the sums are still to be added, whatever their number
+        const SpreadPlan q = take_spread(a, V, true);
+        const long long blocks = groups * q.slabs * q.chunks;
+        if (batch * q.chunks > 0x7fffffffLL) return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many utterances times frames");
+        a.parts = 1;  // the second launch adds the sets of sums itself
+        const long long more = a.grad_weight != nullptr || a.grad_bias != nullptr ? (channels + 31) / 32 : 0;
         if ((rc = launch(who, norm_sums_kernel<T, V>, a, blocks, 1, 0, st, batch)) != MELLIN_OK) return rc;
-        return launch(who, norm_grad_input_kernel<T, V>, a, blocks, 1, 0, st, batch, true);
+        return launch(who, norm_grad_input_kernel<T, V>, a, blocks + more, 1, 0, st, batch, true);
       });
       if (rc != MELLIN_OK || a.parts == 1) return rc;
     }
     if (a.grad_weight == nullptr && a.grad_bias == nullptr) return MELLIN_OK;
     const cudaError_t err = launch_after_predecessor(norm_grad_params_kernel<T>, dim3((unsigned)((channels + 31) / 32)),
-                                                     dim3(kThreads), 0, st, a, sums, parts);
+                                                     dim3(kThreads), 0, st, a, parts);
     if (err != cudaSuccess) return fail(MELLIN_ERR_LAUNCH, std::string(who) + ": " + cudaGetErrorString(err));
     return launched(who);
   });
