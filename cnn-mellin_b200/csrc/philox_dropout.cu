@@ -27,9 +27,8 @@ __device__ __forceinline__ Words philox4x32_10(unsigned long long counter, unsig
   unsigned k0 = (unsigned)key, k1 = (unsigned)(key >> 32);
 #pragma unroll
   for (int round = 0; round < 10; ++round) {
-    const unsigned long long p0 = (unsigned long long)0xD2511F53u * c0, p1 = (unsigned long long)0xCD9E8D57u * c2;
-    c0 = (unsigned)(p1 >> 32) ^ c1 ^ k0, c1 = (unsigned)p1;
-    c2 = (unsigned)(p0 >> 32) ^ c3 ^ k1, c3 = (unsigned)p0;
+    const unsigned h0 = __umulhi(0xD2511F53u, c0), l0 = 0xD2511F53u * c0, h1 = __umulhi(0xCD9E8D57u, c2), l1 = 0xCD9E8D57u * c2;
+    c0 = h1 ^ c1 ^ k0, c1 = l1, c2 = h0 ^ c3 ^ k1, c3 = l0;
     k0 += 0x9E3779B9u, k1 += 0xBB67AE85u;
   }
   return {{c0, c1, c2, c3}};
@@ -47,10 +46,11 @@ struct DropoutArgs {
   const long long *seed_device = nullptr;  // read instead of `seed` when there is one
 };
 
-// Two accesses of 16 bytes a thread are in flight before the generator's work, which then bounds 16-bit tensors: a call has
-// 19 multiplications of 32 by 32 to 64 bits for 4 elements, and the multiplier takes 16 of them a clock and
-// multiprocessor.  26.2 M elements: float32 39 us = 5370 GB/s (0.82 of the measured copy rate), bfloat16 33 us =
-// 3190 GB/s, with a residual 41 us = 3830 GB/s; one or four groups a thread: 43 / 35 / 40 and 41 / 34 / 41 us.
+// Two accesses of 16 bytes a thread are in flight before the generator's work, which then bounds 16-bit tensors: a call for
+// four elements has 38 instructions of the multiplier's pipe and 47 of the integer pipe, each of which takes one every
+// second clock.  26.2 M elements: float32 37 us = 5670 GB/s (0.87 of the measured copy rate), bfloat16 32 us = 3230 GB/s,
+// with a residual 37 us = 4240 GB/s.  With whole 64-bit products 40 / 33 / 41 us; with one or four groups a thread 43 / 35 /
+// 40 and 41 / 34 / 41 us.
 //
 // V elements a group, a multiple of 4; U groups a thread, kThreads groups apart, whose loads are issued together.  VEC:
 // whole groups by packed accesses (aligned; one row of any length, or rows a multiple of V long); the group that ends a
