@@ -15,7 +15,6 @@
 #include <algorithm>
 
 #include "sequence_common.cuh"
-#include "tc_ptx.cuh"
 
 namespace mellin {
 namespace {
@@ -234,6 +233,7 @@ __device__ __forceinline__ void team_sum(A (&v)[Q], int team_id, int team, A (*s
 
 template <typename T, int V, int MB>
 __global__ void __launch_bounds__(kThreads, MB) norm_fused_kernel(const NormArgs<T> a) {
+  begin<true>();
   using A = Acc<T>;
   extern __shared__ __align__(16) unsigned char shared_raw[];
   __shared__ __align__(16) A slots[2][kThreads / 32];
@@ -310,6 +310,7 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_kernel(const NormArgs
 // block has all utterances).
 template <typename T, int V, int MB, bool MANY>
 __global__ void __launch_bounds__(kThreads, MB) norm_fused_backward_kernel(const NormArgs<T> a) {
+  begin<true>();
   using A = Acc<T>;
   extern __shared__ __align__(16) unsigned char shared_raw[];
   __shared__ __align__(16) A slots[2][2][kThreads / 32];
@@ -447,7 +448,7 @@ __device__ __forceinline__ void add_parts(const NormArgs<T> &a, int parts, int b
 //
 // Groups that a cluster's shared memory does not hold.  A block has `tx` packs of channels of one group and `chunk_rows`
 // of its utterance's frames; `slabs` blocks side by side have a frame of the group, `chunks` one after the other its
-// frames.  The first launch writes every block's sums; in the second, which is scheduled while the first drains, every
+// frames.  The first launch writes every block's sums; in the second every
 // block adds its group's and normalises its part, read from L2 as a rule.  4 x 16384 x 256 channels, 8 groups, SiLU,
 // bfloat16: 25 us forward and 42 us backward (bytes alone: 10 and 15); 12 x 548..2191 x 549 float32, one group: 39 and 55
 // (12 and 22).
@@ -500,6 +501,7 @@ __device__ __forceinline__ void walk(const Frames<const T> &xf, const Frames<con
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads, 3) norm_moments_kernel(const NormArgs<T> a) {
+  begin<true>();
   using A = Acc<T>;
   constexpr int U = kSpreadRows<Raw<T, V>::kBytes, false>;
   __shared__ __align__(16) A slots[2][kThreads / 32];
@@ -525,6 +527,7 @@ __global__ void __launch_bounds__(kThreads, 3) norm_moments_kernel(const NormArg
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads, 3) norm_apply_kernel(const NormArgs<T> a) {
+  begin<true>();
   using A = Acc<T>;
   constexpr int U = kSpreadRows<Raw<T, V>::kBytes, false>;
   __shared__ __align__(16) A slots[3][kThreads / 32];
@@ -536,7 +539,6 @@ __global__ void __launch_bounds__(kThreads, 3) norm_apply_kernel(const NormArgs<
     scale[v] = a.weight != nullptr && s.live ? a.weight[s.c + v] : A(1);
     shift[v] = a.bias != nullptr && s.live ? a.bias[s.c + v] : A(0);
   }
-  tc::grid_dependency_wait();  // the sums
   if (s.n >= a.batch) return;
   const A *in = a.part + ((long long)s.n * a.groups + s.g) * a.entries * 3;
   A sums[2] = {A(0), A(0)}, squares[1] = {A(0)};
@@ -578,6 +580,7 @@ __global__ void __launch_bounds__(kThreads, 3) norm_apply_kernel(const NormArgs<
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads, 2) norm_sums_kernel(const NormArgs<T> a) {
+  begin<true>();
   using A = Acc<T>;
   constexpr int U = kSpreadRows<Raw<T, V>::kBytes, true>;
   __shared__ __align__(16) A slots[2][kThreads / 32];
@@ -631,13 +634,13 @@ __global__ void __launch_bounds__(kThreads, 2) norm_sums_kernel(const NormArgs<T
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads, 2) norm_grad_input_kernel(const NormArgs<T> a) {
+  begin<true>();
   using A = Acc<T>;
   constexpr int U = kSpreadRows<Raw<T, V>::kBytes, true>;
   __shared__ __align__(16) A slots[2][kThreads / 32];
   const int parts_of_all = a.groups * a.slabs * a.chunks;
   if ((int)blockIdx.x >= parts_of_all) {  // the blocks behind the parts of the first utterance add the parameters' sums
     if (blockIdx.y != 0 || blockIdx.z != 0) return;
-    tc::grid_dependency_wait();
     add_parts(a, a.batch * a.chunks, (int)blockIdx.x - parts_of_all);
     return;
   }
@@ -651,7 +654,6 @@ __global__ void __launch_bounds__(kThreads, 2) norm_grad_input_kernel(const Norm
     scale[v] = rstd * (a.weight != nullptr && s.live ? a.weight[s.c + v] : A(1));
     bias[v] = a.bias != nullptr && s.live ? a.bias[s.c + v] : A(0);
   }
-  tc::grid_dependency_wait();  // the sums
   const A *in = a.gsums + ((long long)s.n * a.groups + s.g) * a.entries * 2;
   for (int e = threadIdx.x; e < a.entries; e += kThreads) sums[0] += in[2 * e], sums[1] += in[2 * e + 1];
   team_sum(sums, 0, kThreads, slots);
@@ -683,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_grad_input_kernel(const Norm
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) norm_grad_params_kernel(const NormArgs<T> a, int parts) {
-  tc::grid_dependency_wait();
+  begin<true>();
   add_parts(a, parts, (int)blockIdx.x);
 }
 
@@ -813,29 +815,15 @@ SpreadPlan take_spread(NormArgs<T> &a, int V, bool backward) {
 
 template <typename K, typename T>
 int launch(const char *who, K kernel, const NormArgs<T> &a, long long blocks, int cluster, size_t shared, cudaStream_t st,
-           long long utterances, bool after_predecessor = false) {
-  if (blocks > 0x7fffffffLL) return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many blocks");
-  cudaLaunchConfig_t cfg = {};
+           long long utterances) {
   const unsigned planes = (unsigned)((utterances + 65534) / 65535);  // the grid's second extent ends at 65535
-  cfg.gridDim = dim3((unsigned)blocks, (unsigned)std::min<long long>(utterances, 65535), planes);
-  if (planes > 65535) return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many blocks");
-   cfg.blockDim = dim3(kThreads), cfg.stream = st, cfg.dynamicSmemBytes = shared;
+  if (blocks > 0x7fffffffLL || planes > 65535) return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many blocks");
   if (shared > 44 * 1024) {  // with the static arrays beside it: beyond what a launch may have without asking
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 4096);
     if (err != cudaSuccess) return fail(MELLIN_ERR_LAUNCH, std::string(who) + ": " + cudaGetErrorString(err));
   }
-  cudaLaunchAttribute attr[1];
-  cfg.attrs = attr;
-  if (cluster > 1) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.numAttrs = 1;
-  } else if (after_predecessor && dependent_launch_enabled()) {  // the kernel waits for the one before it by itself
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 1;
-  }
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, a);
+  const dim3 grid((unsigned)blocks, (unsigned)std::min<long long>(utterances, 65535), planes);
+  const cudaError_t err = launch_kernel(kernel, grid, kThreads, shared, cluster, st, a);
   if (err != cudaSuccess) return fail(MELLIN_ERR_LAUNCH, std::string(who) + ": " + cudaGetErrorString(err));
   return launched(who);
 }
@@ -894,7 +882,7 @@ int run_forward(NormArgs<T> a, int64_t batch, int64_t frames, int64_t channels, 
       const SpreadPlan q = take_spread(a, V, false);
       const long long blocks = groups * q.slabs * q.chunks;
       if ((rc = launch(who, norm_moments_kernel<T, V>, a, blocks, 1, 0, st, batch)) != MELLIN_OK) return rc;
-      return launch(who, norm_apply_kernel<T, V>, a, blocks, 1, 0, st, batch, true);
+      return launch(who, norm_apply_kernel<T, V>, a, blocks, 1, 0, st, batch);
     });
   });
 }
@@ -929,13 +917,12 @@ int run_backward(NormArgs<T> a, int64_t batch, int64_t frames, int64_t channels,
         a.parts = 1;  // the second launch adds the sets of sums itself
         const long long more = a.grad_weight != nullptr || a.grad_bias != nullptr ? (channels + 31) / 32 : 0;
         if ((rc = launch(who, norm_sums_kernel<T, V>, a, blocks, 1, 0, st, batch)) != MELLIN_OK) return rc;
-        return launch(who, norm_grad_input_kernel<T, V>, a, blocks + more, 1, 0, st, batch, true);
+        return launch(who, norm_grad_input_kernel<T, V>, a, blocks + more, 1, 0, st, batch);
       });
       if (rc != MELLIN_OK || a.parts == 1) return rc;
     }
     if (a.grad_weight == nullptr && a.grad_bias == nullptr) return MELLIN_OK;
-    const cudaError_t err = launch_after_predecessor(norm_grad_params_kernel<T>, dim3((unsigned)((channels + 31) / 32)),
-                                                     dim3(kThreads), 0, st, a, parts);
+    const cudaError_t err = launch_kernel(norm_grad_params_kernel<T>, dim3((unsigned)((channels + 31) / 32)), kThreads, 0, 1, st, a, parts);
     if (err != cudaSuccess) return fail(MELLIN_ERR_LAUNCH, std::string(who) + ": " + cudaGetErrorString(err));
     return launched(who);
   });

@@ -57,6 +57,7 @@ struct DropoutArgs {
 // row which is no multiple of V, and everything without VEC, element by element.
 template <typename T, int V, int U, bool VEC, bool RESIDUAL>
 __global__ void __launch_bounds__(kThreads) philox_dropout_kernel(const DropoutArgs<T> a) {
+  begin<true>();
   using A = Acc<T>;
   const unsigned long long key = a.seed_device != nullptr ? (unsigned long long)*a.seed_device : a.seed;
   const long long total = a.rows * a.cols;
@@ -141,15 +142,16 @@ int run(DropoutArgs<T> a, double p, void *stream) {
                      (a.rows == 1 || (a.cols % V == 0 && a.x_stride % V == 0 && a.r_stride % V == 0));
     const long long per_block = (long long)V * U * kThreads, blocks = (total + per_block - 1) / per_block;
     if (blocks > 0x7fffffffLL) return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": more than 2^42 elements");
-    auto st = static_cast<cudaStream_t>(stream);
+    cudaError_t err = cudaSuccess;
     auto go = [&](auto vector, auto residual) {
-      philox_dropout_kernel<T, V, U, decltype(vector)::value, decltype(residual)::value>
-          <<<(unsigned)blocks, kThreads, 0, st>>>(a);
+      err = launch_kernel(philox_dropout_kernel<T, V, U, decltype(vector)::value, decltype(residual)::value>,
+                          dim3((unsigned)blocks), kThreads, 0, 1, stream, a);
     };
     if (vec && a.residual != nullptr) go(std::true_type{}, std::true_type{});
     else if (vec) go(std::true_type{}, std::false_type{});
     else if (a.residual != nullptr) go(std::false_type{}, std::true_type{});
     else go(std::false_type{}, std::false_type{});
+    if (err != cudaSuccess) return fail(MELLIN_ERR_LAUNCH, std::string(who) + ": " + cudaGetErrorString(err));
     return launched(who);
   });
 }

@@ -43,6 +43,7 @@ struct RecurrenceArgs {
 // for tensors whose frames lie 2^31 elements or more apart.
 template <typename T, int EVERY>
 __global__ void __launch_bounds__(kWalkThreads) recurrence_walk_kernel(const RecurrenceArgs<T> a) {
+  begin<false>();
   using A = Acc<T>;
   const long long i = blockIdx.x * (long long)kWalkThreads + threadIdx.x;
   if (i >= (long long)a.batch * a.channels) return;
@@ -66,6 +67,7 @@ __global__ void __launch_bounds__(kWalkThreads) recurrence_walk_kernel(const Rec
 
 template <typename T, int EVERY>
 __global__ void __launch_bounds__(kWalkThreads) recurrence_walk_backward_kernel(const RecurrenceArgs<T> a) {
+  begin<false>();
   using A = Acc<T>;
   const long long i = blockIdx.x * (long long)kWalkThreads + threadIdx.x;
   if (i >= (long long)a.batch * a.channels) return;
@@ -140,6 +142,7 @@ struct alignas(16) ScanShared {
 };
 template <typename T, int V, int CL, int W, int MB>
 __global__ void __launch_bounds__(32 * W, MB) recurrence_scan_kernel(const RecurrenceArgs<T> a) {
+  begin<false>();
   using A = Acc<T>;
   constexpr int TL = 32 / CL, S = kStateStride / TL, CT = CL * V, SPAN = W * kStateStride;
   __shared__ ScanShared<A, CT, W> sh;
@@ -271,6 +274,7 @@ __global__ void __launch_bounds__(32 * W, MB) recurrence_scan_kernel(const Recur
 // by shuffles.
 template <typename T, int V, int CL, int W, int MB>
 __global__ void __launch_bounds__(32 * W, MB) recurrence_scan_backward_kernel(const RecurrenceArgs<T> a) {
+  begin<false>();
   using A = Acc<T>;
   constexpr int TL = 32 / CL, S = kStateStride / TL, CT = CL * V, SPAN = W * kStateStride;
   __shared__ ScanShared<A, CT, W> sh;
@@ -568,6 +572,7 @@ __device__ __forceinline__ Run run_of(const RecurrenceArgs<T> &a) {
 
 template <typename T, int V, int CL>
 __global__ void __launch_bounds__(32 * kLongWarps, 16 / kLongWarps) recurrence_long_kernel(const RecurrenceArgs<T> a) {
+  begin<false>();
   using A = Acc<T>;
   __shared__ LongShared<A, V * CL> sh;
   const Run r = run_of<T, V, CL>(a);
@@ -624,6 +629,7 @@ __global__ void __launch_bounds__(32 * kLongWarps, 16 / kLongWarps) recurrence_l
 
 template <typename T, int V, int CL>
 __global__ void __launch_bounds__(32 * kLongWarps, 16 / kLongWarps) recurrence_long_backward_kernel(const RecurrenceArgs<T> a) {
+  begin<false>();
   using A = Acc<T>;
   __shared__ LongShared<A, V * CL> sh;
   const Run r = run_of<T, V, CL>(a);
@@ -740,13 +746,7 @@ bool is_long(int64_t batch, int64_t frames, int64_t channels) {
 template <typename K, typename T>
 int launch(const char *who, K kernel, const RecurrenceArgs<T> &a, long long blocks, int threads, void *stream) {
   if (blocks > 0x7fffffffLL) return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": too many utterances times channels");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks), cfg.blockDim = dim3((unsigned)threads), cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)a.cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr, cfg.numAttrs = a.cluster > 1 ? 1 : 0;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, a);
+  const cudaError_t err = launch_kernel(kernel, dim3((unsigned)blocks), threads, 0, a.cluster, stream, a);
   if (err != cudaSuccess) return fail(MELLIN_ERR_LAUNCH, std::string(who) + ": " + cudaGetErrorString(err));
   return launched(who);
 }

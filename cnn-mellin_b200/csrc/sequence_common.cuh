@@ -13,6 +13,7 @@
 
 #include "../../include/mellin_b200.h"
 #include "mellin_internal.h"
+#include "tc_ptx.cuh"
 
 namespace mellin {
 namespace seq {
@@ -263,6 +264,36 @@ __device__ __forceinline__ void sigmoid_pair(double g, double &f, double &keep) 
   const double e = exp(-fabs(g)), r = 1.0 / (1.0 + e), q = e * r;
   f = g < 0.0 ? q : r;
   keep = g < 0.0 ? r : q;
+}
+
+// Every kernel here is launched programmatically dependent: its launch is under way while the kernel before it runs out,
+// and begin() waits for that one before it touches memory.  With EARLY the next kernel's blocks may also take their
+// places as this one's blocks leave: good for many short blocks (dropout 78 -> 76 us, norm 91 -> 88 of the training
+// cases), bad where few long ones should spread evenly (recurrence, decoding: 31 -> 34 us).
+template <bool EARLY>
+__device__ __forceinline__ void begin() {
+  if constexpr (EARLY) tc::launch_dependents();
+  tc::grid_dependency_wait();
+}
+template <typename... KernelArgs, typename... Args>
+cudaError_t launch_kernel(void (*kernel)(KernelArgs...), dim3 grid, int threads, size_t shared, int cluster, void *stream,
+                          Args &&...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid, cfg.blockDim = dim3((unsigned)threads), cfg.dynamicSmemBytes = shared;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr, cfg.numAttrs = 0;
+  if (dependent_launch_enabled()) {  // without it: an ordinary launch
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = (unsigned)cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, KernelArgs(args)...);
 }
 
 // No C++ exception leaves a C entry point.

@@ -439,7 +439,8 @@ int64_t mellin_launch_count(void);
 int mellin_set_tensor_cores(int enable);
 
 /* The first-layer operators launch their helper kernels (weight operands before, plane sum / reduction after the
- * main kernel) programmatically dependent: a kernel's set-up runs under the kernel before it in the stream.  This
+ * main kernel) programmatically dependent: a kernel's set-up runs under the kernel before it in the stream; the sequence
+ * operators launch every kernel so.  This
  * switches that off (0) or on (non-zero) process-wide and returns the previous setting; off, every launch is an
  * ordinary one.  The environment variable MELLIN_DEPENDENT_LAUNCH=0, read on first use, does the same.  No
  * reference counterpart. */

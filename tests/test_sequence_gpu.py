@@ -527,6 +527,49 @@ def test_other_stream_and_captured_graph(frames):
         assert all(torch.equal(a, c) for a, c in zip(captured, want)), k
 
 
+def test_results_of_two_streams_joined():
+    """An operator that takes what another stream's operator writes, after an event: launched dependent on the kernel before
+    it in its own stream, it still waits for the other stream, eagerly and in a captured graph."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(8, 3000, 256, device="cuda", generator=gen)
+    small = torch.randn(8, 3000, 256, device="cuda", generator=gen)
+    side = torch.cuda.Stream()
+
+    def step(x):
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            a = x
+            for k in range(6):  # long enough to be running still when the other branch is done
+                a = sequence.philox_dropout(a, 0.1, True, k)
+            a, _ = sequence.gated_recurrence(a, a)
+        b = sequence.group_norm_act(small, 4)
+        here.wait_stream(side)
+        return sequence.philox_dropout(a, 0.2, True, 9, b)
+
+    def in_order(x):
+        for k in range(6):
+            x = sequence.philox_dropout(x, 0.1, True, k)
+        x, _ = sequence.gated_recurrence(x, x)
+        torch.cuda.synchronize()
+        return sequence.philox_dropout(x, 0.2, True, 9, sequence.group_norm_act(small, 4))
+
+    want = in_order(x)
+    for _ in range(5):
+        got = step(x)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    static, graph = x.clone(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured = step(static)
+    for k in range(5):
+        static.copy_(x * (k + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, in_order(x * (k + 1))), k
+
+
 def test_entry_points_with_strides_of_the_callers():
     """The C ABI from raw pointers: time running backwards through a negative stride, states off the 16-byte grid."""
     import ctypes
@@ -574,6 +617,24 @@ def test_autocast_meets_in_the_wider_type():
         assert sequence.philox_dropout(x.bfloat16(), 0.5, True, 1, x).dtype == torch.float32
         assert sequence.gated_recurrence(x.bfloat16(), x)[0].dtype == torch.float32
         assert sequence.group_norm_act(x.bfloat16(), 2).dtype == torch.bfloat16
+
+
+def test_ordinary_launches_give_the_same():
+    """The switch that turns dependent launches off changes no bit."""
+    x = torch.randn(3, 2600, 64, device="cuda", requires_grad=True)
+    w = torch.randn(64, device="cuda", requires_grad=True)
+
+    def step():
+        y, final = sequence.gated_recurrence(x, x)
+        z = sequence.philox_dropout(sequence.group_norm_act(y, 2, w, activation="gelu"), 0.3, True, 4, y)
+        return [z.detach(), final.detach()] + list(torch.autograd.grad(z.square().sum(), [x, w]))
+
+    first = step()
+    before = capi.set_dependent_launch(False)
+    try:
+        assert all(torch.equal(a, b) for a, b in zip(first, step()))
+    finally:
+        capi.set_dependent_launch(before)
 
 
 def test_launches():
