@@ -188,7 +188,8 @@ __device__ __forceinline__ void add_batch(Moments<Acc<T>> &m, int n, F &&frame) 
     }
   }
   const A count = A(n * V), off = sum * reciprocal_unit(count);
-  join(m.mean, m.m2, m.count, pivot + off, max(squares - sum * off, A(0)), count);
+  // squares beyond the type's range become NaN here, not a variance of zero
+  join(m.mean, m.m2, m.count, pivot + off, max_nan(squares - sum * off, A(0)), count);
 }
 
 // A cluster's barrier in two halves: what lies between them does not wait for blocks that have not started
@@ -690,7 +691,6 @@ __global__ void __launch_bounds__(kThreads) norm_grad_params_kernel(const NormAr
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
-
 
 // Shared memory of a fused kernel's block: two fit a multiprocessor, or three of a forward call in 16 bits (32 utterances
 // of 200 to 800 frames, 1024 channels, 32 groups, SiLU: 27 us against 31; float32 would need twice the clusters, 45

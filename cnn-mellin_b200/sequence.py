@@ -68,7 +68,8 @@ def group_norm_act(
     between the first and the last dimension, or, with ``lens`` and a (batch, frames, channels) input, over the
     utterance's own frames: those behind its end are never read, their outputs and gradients are zero.  ``activation``:
     ``"none"``, ``"relu"``, ``"silu"`` or ``"gelu"`` (with the error function).  Differentiable in input, weight and bias;
-    the parameters' gradients are summed in a fixed order."""
+    the parameters' gradients are summed in a fixed order.  A group whose squared deviations pass the statistics' type
+    (float32 ends at 3.4e38) has no finite variance and comes out as NaN or ``act(bias)``."""
     _on_device("group_norm_act", input)
     if activation not in ACTIVATIONS:
         raise ValueError("group_norm_act: activation must be one of %s, got %r" % (sorted(ACTIVATIONS), activation))

@@ -295,6 +295,20 @@ def test_group_norm_large_mean():
     assert abs(float(y.var(unbiased=False)) - 1) <= 1e-3
 
 
+@pytest.mark.parametrize("frames,channels", [(1, 8), (40, 64), (3000, 512)])
+def test_group_norm_beyond_the_statistics_range(frames, channels):
+    """Squares that pass float32 leave no variance of zero behind: |(x - mean) / std| of n values is at most sqrt(n), so
+    nothing finite may be larger.  The other groups do not notice."""
+    x = torch.randn(2, frames, channels, device="cuda")
+    per = channels // 2
+    wild = x.clone()
+    wild[1, :, per:] *= 3e30
+    y, want = (sequence.group_norm_act(v, 2, activation="none") for v in (wild, x))
+    assert torch.equal(y[0], want[0]) and torch.equal(y[1, :, :per], want[1, :, :per])
+    off = y[1, :, per:]
+    assert not bool((off.abs() > (frames * per) ** 0.5 * (1 + 1e-5)).any())
+
+
 def test_group_norm_other_shapes():
     """(batch, channels), images channels last, 16-bit parameters, no frames, no utterances."""
     gen = torch.Generator(device="cuda").manual_seed(3)
