@@ -26,8 +26,9 @@ CAPI_SOURCES = ["capi.cu", "kernels.cu", "tc_direct.cu", "tc_direct_taps.cu", "t
 CAPI_HEADERS = ["mellin_internal.h", "index_map.h", "tc_ptx.cuh", "tuning_hooks.h"]
 # headers that only some sources include
 EXTRA_DEPS = {"tc_direct_taps.cu": ["tc_direct.cu"], "tc_direct_masked.cu": ["tc_direct.cu"],
-              "recurrence.cu": ["sequence_common.cuh"], "group_norm.cu": ["sequence_common.cuh"],
-              "philox_dropout.cu": ["sequence_common.cuh"]}
+              "recurrence.cu": ["sequence_common.cuh", "sequence_index.h"],
+              "group_norm.cu": ["sequence_common.cuh", "sequence_index.h"],
+              "philox_dropout.cu": ["sequence_common.cuh", "sequence_index.h"]}
 TORCH_SOURCES = ["mellin_torch.cpp", "sequence_torch.cpp"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

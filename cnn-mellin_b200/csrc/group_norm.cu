@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_kernel(const NormArgs
   if (!s.live) return;
   const A rstd = count > A(0) ? A(1) / sqrt(m2 / count + a.eps) : A(0);  // no frames: nothing to scale, no 0 * inf
   if (a.stats_out != nullptr && s.j == 0 && s.rank == 0) {
-    A *out = a.stats_out + (s.n * a.groups + s.g) * 2;
+    A *out = a.stats_out + stats_offset(s.n, a.groups, s.g);
     out[0] = mean, out[1] = rstd;
   }
 #pragma unroll
@@ -346,7 +346,10 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_backward_kernel(const
     }
     if (s.live) clear_from<T, V>(a.grad_x, n, s.c, len + s.row_rank * s.rows + s.ty, a.row_ranks * s.rows, a.frames);
     A mean = 0, rstd = 0, scale[V], q1[V], q2[V], sums[2] = {A(0), A(0)};
-    if (s.live) mean = a.stats[(n * a.groups + s.g) * 2], rstd = a.stats[(n * a.groups + s.g) * 2 + 1];
+    if (s.live) {
+      const A *st = a.stats + stats_offset(n, a.groups, s.g);
+      mean = st[0], rstd = st[1];
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) q1[v] = q2[v] = 0, scale[v] = rstd * weight[v];
     by_act(a.act, [&](auto act) {
@@ -553,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 3) norm_apply_kernel(const NormArgs<
   team_sum(squares, 0, kThreads, &slots[2]);
   const A rstd = count > A(0) ? A(1) / sqrt(squares[0] / count + a.eps) : A(0);
   if (a.stats_out != nullptr && s.entry == 0 && threadIdx.x == 0) {
-    A *out = a.stats_out + ((long long)s.n * a.groups + s.g) * 2;
+    A *out = a.stats_out + stats_offset(s.n, a.groups, s.g);
     out[0] = mean, out[1] = rstd;
   }
   if (!s.live) return;
@@ -589,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_sums_kernel(const NormArgs<T
   const Part s = part_of<T, V>(a);
   if (s.n >= a.batch) return;
   const int end = s.live ? min(s.end, s.len) : 0, first = s.begin + s.ty;
-  const A *st = a.stats + ((long long)s.n * a.groups + s.g) * 2, mean = st[0], rstd = st[1];
+  const A *st = a.stats + stats_offset(s.n, a.groups, s.g), mean = st[0], rstd = st[1];
   A scale[V], weight[V], bias[V], q1[V], q2[V], sums[2] = {A(0), A(0)};
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -648,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_grad_input_kernel(const Norm
   const Part s = part_of<T, V>(a);
   if (s.n >= a.batch) return;
   const int end = s.live ? min(s.end, s.len) : 0, first = s.begin + s.ty;
-  const A *st = a.stats + ((long long)s.n * a.groups + s.g) * 2, mean = st[0], rstd = st[1];
+  const A *st = a.stats + stats_offset(s.n, a.groups, s.g), mean = st[0], rstd = st[1];
   A scale[V], bias[V], sums[2] = {A(0), A(0)};
 #pragma unroll
   for (int v = 0; v < V; ++v) {

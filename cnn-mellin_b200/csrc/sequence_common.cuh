@@ -13,6 +13,7 @@
 
 #include "../../include/mellin_b200.h"
 #include "mellin_internal.h"
+#include "sequence_index.h"
 #include "tc_ptx.cuh"
 
 namespace mellin {

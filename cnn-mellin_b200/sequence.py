@@ -69,7 +69,8 @@ def group_norm_act(
     utterance's own frames: those behind its end are never read, their outputs and gradients are zero.  ``activation``:
     ``"none"``, ``"relu"``, ``"silu"`` or ``"gelu"`` (with the error function).  Differentiable in input, weight and bias;
     the parameters' gradients are summed in a fixed order.  A group whose squared deviations pass the statistics' type
-    (float32 ends at 3.4e38) has no finite variance and comes out as NaN or ``act(bias)``."""
+    (float32 ends at 3.4e38) has no finite variance and comes out as NaN or ``act(bias)``.  Batch times channels is below
+    2^31."""
     _on_device("group_norm_act", input)
     if activation not in ACTIVATIONS:
         raise ValueError("group_norm_act: activation must be one of %s, got %r" % (sorted(ACTIVATIONS), activation))
@@ -141,7 +142,8 @@ class GatedRecurrence(torch.nn.Module):
 class GroupNormAct(torch.nn.Module):
     """:func:`group_norm_act` with learnable ``weight`` and ``bias`` (names and shapes of ``torch.nn.GroupNorm``).
 
-    ``per_frame``: the statistics of each frame by itself, as a stream that comes in pieces needs them."""
+    ``per_frame``: the statistics of each frame by itself, as a stream that comes in pieces needs them (the frames are then
+    the batch: utterances times frames times channels is below 2^31)."""
 
     def __init__(self, num_groups: int, num_channels: int, activation: str = "relu", eps: float = 1e-5,
                  per_frame: bool = False):

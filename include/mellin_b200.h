@@ -303,8 +303,9 @@ int mellin_lift_compress_backward_f64(const double *x, const double *grad_y, con
  * gradients are written as zeros.  Suffixes f32 / f64 / f16 / bf16 name the tensors' type (`const void *` = device
  * pointers to IEEE half / bfloat16 values); sums, states, statistics and parameters are float (double for f64).  No
  * call allocates, blocks or synchronises: all of them can be captured into a graph.  Frames and channels are at most
- * 2^30 each.  No reference counterpart: the
- * reference's AcousticModel uses torch's recurrent layers and dropout there (models.py:435-445). */
+ * 2^30 each, and batch times channels of the group norm is below 2^31 (a norm of each frame by itself, whose batch is
+ * utterances times frames, meets that first).  No reference counterpart: the reference's AcousticModel uses torch's
+ * recurrent layers and dropout there (models.py:435-445). */
 
 /* Gated linear recurrence: f = sigmoid(gate), h_t = f_t h_{t-1} + (1 - f_t) x_t, y_t = h_t, over an utterance's frames,
  * first to last or (reverse != 0) last to first.  initial: (batch, channels) state before the first frame met, or

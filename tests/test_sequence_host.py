@@ -140,3 +140,27 @@ def test_block_parameters():
     one_way = sequence.SequenceBlock(64, 32, num_groups=4, streaming=True)
     assert one_way.recurrence.directions == 1 and one_way.norm.per_frame
     assert "hidden=32" in repr(block) and "p=0.05" in repr(block)
+
+
+def test_statistics_offsets_beyond_32_bits(tmp_path):
+    """The kernels' offset into (batch, groups, 2) statistics, compiled for the host, at the largest extents that the entry
+    points admit (batch * groups below 2^31): no launch of that size is needed to see it wrap."""
+    import os
+    import re
+    import subprocess
+
+    csrc = os.path.join(os.path.dirname(os.path.abspath(capi.__file__)), "csrc")
+    source = tmp_path / "offset.cpp"
+    source.write_text('#include "sequence_index.h"\n'
+                      'extern "C" long long offset(int n, int groups, int g) { return mellin::seq::stats_offset(n, groups, g); }\n')
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-I", csrc, str(source), "-o", str(tmp_path / "offset.so")],
+                   check=True)
+    offset = ctypes.CDLL(str(tmp_path / "offset.so")).offset
+    offset.restype, offset.argtypes = ctypes.c_longlong, [ctypes.c_int] * 3
+    for batch, groups in ((1, 1), (3, 32), (2 ** 20, 1024), (2 ** 21 - 1, 1024), (1, 2 ** 30), (2 ** 31 - 1, 1), (46340, 46341)):
+        for n, g in ((0, 0), (batch - 1, 0), (batch - 1, groups - 1), (batch // 2, groups // 2)):
+            assert offset(n, groups, g) == (n * groups + g) * 2
+    # and every access to the statistics in the kernels goes through it
+    text = open(os.path.join(csrc, "group_norm.cu")).read()
+    uses = re.findall(r"a\.stats(?:_out)? \+ (\w+)|a\.stats(?:_out)?(\[)", text)
+    assert len(uses) == 5 and all(use == ("stats_offset", "") for use in uses)
