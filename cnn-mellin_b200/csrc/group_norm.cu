@@ -95,11 +95,22 @@ struct NormArgs {
 template <typename A>
 __device__ __forceinline__ void join(A &mean, A &m2, A &count, A mean_b, A m2_b, A count_b) {
   if (count_b == A(0)) return;
+  if (count == A(0)) {  // taken over as they are: the square of a mean far from zero may pass the type's range
+    mean = mean_b, m2 = m2_b, count = count_b;
+    return;
+  }
   const A total = count + count_b, delta = mean_b - mean, share = count_b * reciprocal_unit(total);
   mean += delta * share;
   m2 += m2_b + delta * delta * count * share;
   count = total;
 }
+
+// Sums of count * mean are formed 2^32 times smaller: that changes no bit of them (unless the mean is below 1e-28) and keeps
+// those of large groups within the type's range where the mean is.
+template <typename A>
+constexpr A kShrink = A(1) / A(4294967296.0);
+template <typename A>
+constexpr A kGrow = A(4294967296.0);
 
 // ---- one pass: a group's values stay in shared memory between the sums and the result ---------------------------------
 //
@@ -266,9 +277,9 @@ __global__ void __launch_bounds__(kThreads, MB) norm_fused_kernel(const NormArgs
 
   // the block's: sum of the values, then of the squared deviations from their mean
   A count = A(span.end - span.begin) * A(s.some ? s.cols * V : 0);
-  A total[1] = {m.count * m.mean};
+  A total[1] = {m.count * (m.mean * kShrink<A>)};
   team_sum(total, s.team_id, a.team, &slots[0]);
-  A mean = count > A(0) ? total[0] / count : A(0);
+  A mean = count > A(0) ? total[0] / count * kGrow<A> : A(0);
   const A d = m.mean - mean;
   A squares[1] = {m.m2 + m.count * d * d};
   team_sum(squares, s.team_id, a.team, &slots[1]);
@@ -518,9 +529,9 @@ __global__ void __launch_bounds__(kThreads, 3) norm_moments_kernel(const NormArg
                       add_batch<T, V, U>(m, n, [&](int i) { return xq[i]; });
                     });
   const A count = A(max(end - s.begin, 0)) * A(s.cols * V);
-  A total[1] = {m.count * m.mean};
+  A total[1] = {m.count * (m.mean * kShrink<A>)};
   team_sum(total, 0, kThreads, &slots[0]);
-  const A mean = count > A(0) ? total[0] / count : A(0), d = m.mean - mean;
+  const A mean = count > A(0) ? total[0] / count * kGrow<A> : A(0), d = m.mean - mean;
   A squares[1] = {m.m2 + m.count * d * d};
   team_sum(squares, 0, kThreads, &slots[1]);
   if (threadIdx.x == 0) {
@@ -546,9 +557,9 @@ __global__ void __launch_bounds__(kThreads, 3) norm_apply_kernel(const NormArgs<
   if (s.n >= a.batch) return;
   const A *in = a.part + ((long long)s.n * a.groups + s.g) * a.entries * 3;
   A sums[2] = {A(0), A(0)}, squares[1] = {A(0)};
-  for (int e = threadIdx.x; e < a.entries; e += kThreads) sums[0] += in[3 * e + 2], sums[1] += in[3 * e + 2] * in[3 * e];
+  for (int e = threadIdx.x; e < a.entries; e += kThreads) sums[0] += in[3 * e + 2], sums[1] += in[3 * e + 2] * (in[3 * e] * kShrink<A>);
   team_sum(sums, 0, kThreads, &slots[0]);
-  const A count = sums[0], mean = count > A(0) ? sums[1] / count : A(0);
+  const A count = sums[0], mean = count > A(0) ? sums[1] / count * kGrow<A> : A(0);
   for (int e = threadIdx.x; e < a.entries; e += kThreads) {
     const A d = in[3 * e] - mean;
     squares[0] += in[3 * e + 1] + in[3 * e + 2] * d * d;

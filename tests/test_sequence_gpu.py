@@ -309,6 +309,36 @@ def test_group_norm_beyond_the_statistics_range(frames, channels):
     assert not bool((off.abs() > (frames * per) ** 0.5 * (1 + 1e-5)).any())
 
 
+@pytest.mark.parametrize("frames,channels,std", [(1, 8, 1e17), (5, 64, 1e17), (40, 64, 1e17), (700, 256, 1e16), (3000, 512, 1e16)])
+def test_group_norm_far_mean_within_the_range(frames, channels, std):
+    """Values about 1e20, whose squares pass float32 while their squared deviations do not: in the forms that one team, a
+    block, a cluster and two launches have.
+
+    The mean of values of one size is off by at most 16 of its units (a few joins and a short tree), that is 16 * 2^-24 * 1e20
+    / std of a standard deviation; the normalised values move by that much alike, the variance by its square, and float32
+    rounds a few times at values below 6."""
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    x = (1e20 + std * torch.randn(2, frames, channels, device="cuda", dtype=torch.float64, generator=gen)).float()
+    grad = torch.randn(2, frames, channels, device="cuda", generator=gen)
+    want = so.group_norm_act(_np(x), 2, act="none", grad_y=_np(grad))
+    x.requires_grad_(True)
+    y = sequence.group_norm_act(x, 2, activation="none")
+    _close(y, want["y"], torch.float32, "y")
+    off = 16 * 2 ** -24 * 1e20 / std
+    assert np.abs(_np(y) - want["y"][0]).max() <= off + 6 * off ** 2 + 64 * 2 ** -24
+    _close(torch.autograd.grad(y, x, grad)[0], want["grad_x"], torch.float32, "grad_x")
+
+
+@pytest.mark.parametrize("value", [1e19, -3e19, 1e30, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("frames,channels", [(1, 8), (40, 64), (3000, 512)])
+def test_group_norm_of_one_value(frames, channels, value):
+    """A group that holds one value throughout, up to the type's lowest: sums of the values pass the type, the mean does not.
+    The normalised values are the mean's rounding over itself at most, never NaN."""
+    x = torch.full((2, frames, channels), value, device="cuda", requires_grad=True)
+    y = sequence.group_norm_act(x, 2, activation="none")
+    assert torch.isfinite(y).all() and torch.isfinite(torch.autograd.grad(y.sum(), x)[0]).all()
+
+
 def test_group_norm_other_shapes():
     """(batch, channels), images channels last, 16-bit parameters, no frames, no utterances."""
     gen = torch.Generator(device="cuda").manual_seed(3)
