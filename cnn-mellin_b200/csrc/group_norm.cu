@@ -42,11 +42,20 @@ __device__ __forceinline__ void by_act(int act, F &&body) {
   else body(ActTag<kNone>{});
 }
 
+// SiLU and its slope vanish far below zero, where z sigmoid(z) as a product would not: the least sigmoid in float is
+// 2^-126, which z beyond 1e30 makes visible, and infinity times zero is none.  z sigmoid(z) at the floor is below 2e-36 in
+// size (float) and zero (double).
+template <typename A>
+__device__ __forceinline__ A silu_floor(A z) {
+  return max_nan(z, sizeof(A) == 4 ? A(-128) : A(-1024));
+}
+
 template <typename A>
 __device__ __forceinline__ A act_value(A z, int act) {
   if (act == kRelu) return max_nan(z, A(0));
   if (act == kSilu) {
     A f, keep;
+    z = silu_floor(z);
     sigmoid_pair(z, f, keep);
     return z * f;
   }
@@ -58,6 +67,7 @@ __device__ __forceinline__ A act_slope(A z, int act) {
   if (act == kRelu) return z > A(0) ? A(1) : A(0);
   if (act == kSilu) {
     A f, keep;
+    z = silu_floor(z);
     sigmoid_pair(z, f, keep);
     return f * (A(1) + z * keep);
   }

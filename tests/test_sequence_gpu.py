@@ -339,6 +339,30 @@ def test_group_norm_of_one_value(frames, channels, value):
     assert torch.isfinite(y).all() and torch.isfinite(torch.autograd.grad(y.sum(), x)[0]).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_silu_far_below_zero(dtype):
+    """SiLU and its slope are nothing at z = -200 and below, down to the type's lowest value and -infinity: at most
+    128 * 2^-126 = 1.6e-36 in float32 arithmetic.  The other channels do not notice."""
+    state = torch.float64 if dtype == torch.float64 else torch.float32
+    lowest = torch.finfo(state).min
+    for frames in (3, 40, 3000):
+        x = torch.randn(2, frames, 512, device="cuda").to(dtype).requires_grad_(True)
+        bias = torch.zeros(512, dtype=state, device="cuda")
+        plain = sequence.group_norm_act(x, 2, None, bias, activation="silu")
+        bias[::8] = torch.tensor([-200.0, -1e10, -1e30, -1e37, lowest / 2, lowest, float("-inf"), -1e35], device="cuda",
+                                 dtype=state).repeat(8)
+        bias.requires_grad_(True)
+        y = sequence.group_norm_act(x, 2, None, bias, activation="silu")
+        far = torch.zeros(512, dtype=torch.bool, device="cuda")
+        far[::8] = True
+        assert float(y[..., far].detach().abs().max()) <= 1.6e-36 and torch.equal(y[..., ~far], plain[..., ~far])
+        grad = torch.zeros_like(y)
+        grad[..., far] = 1
+        gx, gb = torch.autograd.grad(y, [x, bias], grad)
+        # slopes below 1.6e-36, summed over at most 2 x 3000 frames, times 1 / std = 1 for the input's gradient
+        assert float(gb.abs().max()) <= 6000 * 1.6e-36 and float(gx.abs().max()) <= 6000 * 1.6e-36
+
+
 def test_group_norm_other_shapes():
     """(batch, channels), images channels last, 16-bit parameters, no frames, no utterances."""
     gen = torch.Generator(device="cuda").manual_seed(3)
