@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(kWalkThreads) recurrence_walk_kernel(const Rec
     if (a.states != nullptr && s % EVERY == 0) a.states[(n * slots + s / EVERY) * a.channels + c] = h;
     const long long t = a.reverse ? len - 1 - s : s;
     A f, keep;
-    sigmoid_pair(to_acc(gate[t * a.gate.st]), f, keep);
+    sigmoid_pair<true>(to_acc(gate[t * a.gate.st]), f, keep);
     h = f * h + keep * to_acc(x[t * a.x.st]);
     y[t * a.y.st] = from_acc<T>(h);
   }
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kWalkThreads) recurrence_walk_backward_kernel(
       if (first + k < len) {
         const long long t = a.reverse ? len - 1 - (first + k) : first + k;
         const A xv = to_acc(x[t * a.x.st]);
-        sigmoid_pair(to_acc(gate[t * a.gate.st]), f[k], keep[k]);
+        sigmoid_pair<true>(to_acc(gate[t * a.gate.st]), f[k], keep[k]);
         d[k] = h - xv;
         h = f[k] * h + keep[k] * xv;
       }
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(32 * W, MB) recurrence_scan_kernel(const Recur
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         A keep;
-        sigmoid_pair(element(gr[j], v), f[j][v], keep);
+        sigmoid_pair<true>(element(gr[j], v), f[j][v], keep);
         u[j][v] = keep * element(xr[j], v);
       }
     if (k + 1 < steps) fetch(k + 1);
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(32 * W, MB) recurrence_scan_backward_kernel(co
       pa[v] = A(1), pb[v] = A(0);
 #pragma unroll
       for (int j = 0; j < S; ++j) {
-        sigmoid_pair(element(gr[j], v), f[j][v], keep[j][v]);
+        sigmoid_pair<true>(element(gr[j], v), f[j][v], keep[j][v]);
         d[j][v] = element(xr[j], v);
         pb[v] = f[j][v] * pb[v] + keep[j][v] * d[j][v], pa[v] *= f[j][v];
       }
@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(32 * kLongWarps, 16 / kLongWarps) recurrence_l
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         A f, keep;
-        sigmoid_pair(element(gr[j], v), f, keep);
+        sigmoid_pair<true>(element(gr[j], v), f, keep);
         pb[v] = f * pb[v] + keep * element(xr[j], v), pa[v] *= f;
       }
   }
@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(32 * kLongWarps, 16 / kLongWarps) recurrence_l
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         A f, keep;
-        sigmoid_pair(element(gr[j], v), f, keep);
+        sigmoid_pair<true>(element(gr[j], v), f, keep);
         h[v] = f * h[v] + keep * element(xr[j], v);
       }
       if (s + j < r.end) store_raw<T, V>(py + (long long)step * j, rounded<T, V>(h));
@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(32 * kLongWarps, 16 / kLongWarps) recurrence_l
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         A f, keep;
-        sigmoid_pair(element(gr[j], v), f, keep);
+        sigmoid_pair<true>(element(gr[j], v), f, keep);
         pb[v] = f * (pb[v] + element(yr[j], v)), pa[v] *= f;
       }
   }
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(32 * kLongWarps, 16 / kLongWarps) recurrence_l
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const A xv = element(xr[j], v);
-        sigmoid_pair(element(gr[j], v), f[j][v], keep[j][v]);
+        sigmoid_pair<true>(element(gr[j], v), f[j][v], keep[j][v]);
         d[j][v] = h[v] - xv;
         h[v] = f[j][v] * h[v] + keep[j][v] * xv;
       }

@@ -253,14 +253,17 @@ __device__ __forceinline__ double max_nan(double a, double b) { return a > b ? a
 
 // sigmoid(g) and 1 - sigmoid(g), each to a few units in its own last place: the complement is e sigmoid(g) with
 // e = exp(-g), not a difference.  e is held at 2^126, so that the quotient stays a normal number (the least sigmoid is
-// 2^-126); NaN stays NaN.
+// 2^-126); NaN stays NaN.  SHUT: where e is held, sigmoid is 0, so that a shut gate lets nothing of a state through whatever
+// its size (2^-126 of 3e38 would be 4); 1 % of the recurrence's time.
+template <bool SHUT = false>
 __device__ __forceinline__ void sigmoid_pair(float g, float &f, float &keep) {
   float t;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(t) : "f"(g * -1.4426950408889634f), "f"(126.f));
-  const float e = exp2_unit(t);
-  f = reciprocal_unit(1.f + e);
-  keep = e * f;
+  const float e = exp2_unit(t), r = reciprocal_unit(1.f + e);
+  keep = e * r;
+  f = SHUT && t >= 126.f ? 0.f : r;
 }
+template <bool SHUT = false>
 __device__ __forceinline__ void sigmoid_pair(double g, double &f, double &keep) {
   const double e = exp(-fabs(g)), r = 1.0 / (1.0 + e), q = e * r;
   f = g < 0.0 ? q : r;

@@ -184,6 +184,27 @@ def test_recurrence_extreme_gates():
         assert torch.isfinite(gx).all() and float(gg.abs().max()) <= 1.01 * least * 480 * 480
 
 
+@pytest.mark.parametrize("frames", [3, 40, 600])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64], ids=str)
+def test_recurrence_shut_gate_behind_a_huge_state(frames, dtype):
+    """A gate of -infinity (or the type's lowest value, or far enough below zero) takes its frame's value alone, whatever
+    finite value the state had; and its gradient passes nothing back."""
+    huge = torch.finfo(dtype).min
+    x = torch.ones(2, frames, 8, device="cuda", dtype=dtype)
+    x[:, ::2] = huge
+    # -200: exp(-200) is 0 beside any float, and 1e-87 in double, where a huge state would show
+    shut = [float("-inf"), torch.finfo(dtype).min, -1e5, -200.0 if dtype != torch.float64 else -1e5]
+    gate = torch.tensor(shut * 2, device="cuda", dtype=dtype).expand(2, frames, 8).contiguous()
+    x.requires_grad_(True), gate.requires_grad_(True)
+    initial = torch.full((2, 8), torch.finfo(torch.float64 if dtype == torch.float64 else torch.float32).min, device="cuda",
+                         dtype=torch.float64 if dtype == torch.float64 else torch.float32, requires_grad=True)
+    for reverse in (False, True):
+        y, final = sequence.gated_recurrence(x, gate, initial, reverse=reverse)
+        assert torch.equal(y, x)
+        gx, gg, gi = torch.autograd.grad([y, final], [x, gate, initial], [torch.ones_like(y), torch.zeros_like(final)])
+        assert torch.equal(gx, torch.ones_like(gx)) and not gg.any() and not gi.any()
+
+
 def test_recurrence_strides_beyond_32_bits():
     """Frames 2^30 elements apart: the offsets pass 32 bits."""
     flat = torch.zeros(5 * 2 ** 30 + 64, dtype=torch.bfloat16, device="cuda")
