@@ -124,8 +124,13 @@ tensor_list once_differentiable(const char *what, tensor_list grads) {
   return grads;
 }
 
-bool wants_grad(const Tensor &t) { return t.requires_grad(); }
-bool wants_grad(const OptTensor &t) { return t && t->requires_grad(); }
+// Whether a call is differentiated with regard to any of its operands.  Forward mode counts, which needs neither
+// requires_grad nor grad mode: there is none here, and the autograd function says so, where its kernels alone would drop the
+// tangents.
+bool differentiated(const Tensor &t) {
+  return (at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined();
+}
+bool differentiated(const OptTensor &t) { return t && differentiated(*t); }
 
 // ---- gated recurrence -----------------------------------------------------------------------------------------------
 
@@ -230,7 +235,7 @@ class GatedRecurrenceFunction : public torch::autograd::Function<GatedRecurrence
 
 std::tuple<Tensor, Tensor> gated_recurrence_autograd(const Tensor &input, const OptTensor &gate, const OptTensor &initial,
                                                      const OptTensor &lens, bool reverse) {
-  if (at::GradMode::is_enabled() && (wants_grad(input) || wants_grad(gate) || wants_grad(initial))) {
+  if (differentiated(input) || differentiated(gate) || differentiated(initial)) {
     auto out = GatedRecurrenceFunction::apply(input, gate, initial, lens, reverse);
     return {out[0], out[1]};
   }
@@ -335,7 +340,7 @@ Tensor group_norm_act_cuda(const Tensor &input, int64_t groups, const OptTensor 
 
 Tensor group_norm_act_autograd(const Tensor &input, int64_t groups, const OptTensor &weight, const OptTensor &bias,
                                const OptTensor &lens, double eps, int64_t act) {
-  if (at::GradMode::is_enabled() && (wants_grad(input) || wants_grad(weight) || wants_grad(bias))) {
+  if (differentiated(input) || differentiated(weight) || differentiated(bias)) {
     const Tensor y = GroupNormActFunction::apply(as_frames("group_norm_act", input, lens), groups, weight, bias, lens, eps, act);
     return input.dim() == 3 ? y : y.reshape(input.sizes());
   }
@@ -425,7 +430,7 @@ class PhiloxDropoutFunction : public torch::autograd::Function<PhiloxDropoutFunc
 
 Tensor philox_dropout_autograd(const Tensor &input, double p, int64_t seed, const OptTensor &seed_tensor,
                                const OptTensor &residual) {
-  if (at::GradMode::is_enabled() && (wants_grad(input) || wants_grad(residual)))
+  if (differentiated(input) || differentiated(residual))
     return PhiloxDropoutFunction::apply(input, p, seed, seed_tensor, residual);
   at::AutoDispatchBelowADInplaceOrView guard;
   return philox_dropout_cuda(input, p, seed, seed_tensor, residual);

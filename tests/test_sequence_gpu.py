@@ -530,6 +530,27 @@ def test_no_second_derivative():
             g.sum().backward()
 
 
+def test_no_forward_mode():
+    """A tangent on any operand is refused, with and without grad mode, never dropped."""
+    import torch.autograd.forward_ad as fwd
+
+    x, row = torch.randn(2, 4, 6, device="cuda"), torch.randn(2, 6, device="cuda")
+    calls = [lambda t: sequence.gated_recurrence(t(x))[0], lambda t: sequence.gated_recurrence(x, t(x))[0],
+             lambda t: sequence.gated_recurrence(x, x, t(row))[0], lambda t: sequence.group_norm_act(t(x), 2),
+             lambda t: sequence.group_norm_act(x, 2, t(row[0])), lambda t: sequence.group_norm_act(x, 2, None, t(row[0])),
+             lambda t: sequence.philox_dropout(t(x), 0.5), lambda t: sequence.philox_dropout(x, 0.5, residual=t(x)),
+             lambda t: sequence.philox_dropout(x, 0.5, False, residual=t(x)), lambda t: sequence.group_norm_act(t(row), 2)]
+    for call in calls:
+        for grad_mode in (True, False):
+            with fwd.dual_level(), torch.set_grad_enabled(grad_mode), pytest.raises(RuntimeError, match="jvp is not implemented"):
+                call(lambda v: fwd.make_dual(v, torch.ones_like(v)))
+        call(lambda v: v)  # and nothing is left behind
+    for f in (lambda v: sequence.gated_recurrence(v)[0], lambda v: sequence.group_norm_act(v, 2),
+              lambda v: sequence.philox_dropout(v, 0.5)):
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (x,), (torch.ones_like(x),))
+
+
 def test_refusals():
     x = torch.randn(2, 4, 6, device="cuda")
     lens = torch.tensor([1, 2], dtype=torch.int32, device="cuda")
