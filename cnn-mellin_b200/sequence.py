@@ -139,11 +139,20 @@ class GatedRecurrence(torch.nn.Module):
         return torch.cat((y0, y1), 2), torch.stack((f0, f1))
 
 
+def _present(x: torch.Tensor, lens: torch.Tensor) -> torch.Tensor:
+    """1 for each of x's frames, one after the other, that is inside its utterance, else 0."""
+    if x.dim() != 3:
+        raise RuntimeError("GroupNormAct: 'lens' goes with a (batch, frames, channels) input")
+    if not lens.is_cuda or lens.dtype != torch.int32 or lens.shape != x.shape[:1] or lens.device != x.device:
+        raise RuntimeError("GroupNormAct: 'lens' must be an int32 CUDA tensor on the input's device with one length per utterance")
+    return (torch.arange(x.shape[1], dtype=torch.int32, device=x.device) < lens[:, None]).int().reshape(-1)
+
+
 class GroupNormAct(torch.nn.Module):
     """:func:`group_norm_act` with learnable ``weight`` and ``bias`` (names and shapes of ``torch.nn.GroupNorm``).
 
     ``per_frame``: the statistics of each frame by itself, as a stream that comes in pieces needs them (the frames are then
-    the batch: utterances times frames times channels is below 2^31)."""
+    the batch: utterances times frames times channels is below 2^31).  ``lens`` as in :func:`group_norm_act` either way."""
 
     def __init__(self, num_groups: int, num_channels: int, activation: str = "relu", eps: float = 1e-5,
                  per_frame: bool = False):
@@ -162,8 +171,9 @@ class GroupNormAct(torch.nn.Module):
 
     def forward(self, x: torch.Tensor, lens: Optional[torch.Tensor] = None) -> torch.Tensor:
         if self.per_frame:
-            y = group_norm_act(x.reshape(-1, x.shape[-1]), self.num_groups, self.weight, self.bias, None, self.eps,
-                               self.activation)
+            rows = x.reshape(-1, 1, x.shape[-1])  # every frame an utterance of its own, which is there (1) or not (0)
+            y = group_norm_act(rows, self.num_groups, self.weight, self.bias, None if lens is None else _present(x, lens),
+                               self.eps, self.activation)
             return y.view(x.shape)
         return group_norm_act(x, self.num_groups, self.weight, self.bias, lens, self.eps, self.activation)
 

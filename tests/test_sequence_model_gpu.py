@@ -70,6 +70,47 @@ def test_block_against_plain_operations(streaming):
     assert state.shape == (1 if streaming else 2, 3, 20)
 
 
+@pytest.mark.parametrize("streaming", [False, True])
+def test_block_with_padding_that_must_not_be_seen(streaming):
+    """NaN, infinities and the lowest value behind the utterances' ends, zero gradients there: what is inside them, the
+    states and every gradient are those of zero padding."""
+    torch.manual_seed(9)
+    block = sequence.SequenceBlock(24, 20, num_groups=4, dropout=0.3, streaming=streaming).cuda()
+    lens = torch.tensor([40, 0, 23, 45, -2], dtype=torch.int32, device="cuda")
+    inside = torch.arange(40, device="cuda")[None, :, None] < lens[:, None, None]
+    x = torch.randn(5, 40, 24, device="cuda")
+    bad = torch.tensor([float("nan"), float("inf"), float("-inf"), torch.finfo(torch.float32).min], device="cuda").repeat(6)
+    grad = torch.where(inside, torch.randn(5, 40, 24, device="cuda"), 0.0)
+    results = []
+    for padding in (0.0, bad):
+        leaf = torch.where(inside, x, padding).requires_grad_(True)
+        torch.manual_seed(6)
+        y, state = block(leaf, lens)
+        grads = torch.autograd.grad(y, [leaf] + list(block.parameters()), grad)
+        results.append([torch.where(inside, y, 0.0).detach(), state.detach()] + list(grads))
+    for a, b in zip(*results):
+        assert torch.isfinite(b).all() and torch.equal(a, b)
+
+
+def test_per_frame_norm_with_lengths():
+    """Frames behind an utterance's end are not read and come out as zeros; lengths that do not fit are refused."""
+    norm = sequence.GroupNormAct(3, 12, "gelu", per_frame=True).cuda()
+    x = torch.randn(3, 7, 12, device="cuda")
+    lens = torch.tensor([7, 0, 4], dtype=torch.int32, device="cuda")
+    inside = torch.arange(7, device="cuda")[None, :, None] < lens[:, None, None]
+    whole = norm(x)
+    y = norm(torch.where(inside, x, float("nan")), lens)
+    assert torch.equal(y, torch.where(inside, whole, 0.0))
+    time_major = torch.where(inside, x, float("nan")).transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(norm(time_major, lens), y)
+    assert norm(x[:, :0], lens).shape == (3, 0, 12) and norm(x[:0], lens[:0]).shape == (0, 7, 12)
+    for bad in (lens.long(), lens.cpu(), lens[:1], lens.view(3, 1)):
+        with pytest.raises(RuntimeError, match="lens"):
+            norm(x, bad)
+    with pytest.raises(RuntimeError, match="lens"):
+        norm(x.view(3, 7, 2, 6).reshape(3, 7, 1, 12), lens)
+
+
 def test_stream_in_pieces():
     """A streaming block fed 1, 7, 1, 16, ... frames at a time with its state gives what one call gives, to float32
     rounding: sums over 48 channels and states that forget within ~100 frames, some 1e-5 at values of order one."""
