@@ -91,7 +91,8 @@ def philox_dropout(
     it again.  A dropped element is zero whatever ``input`` holds there.  ``seed``: an integer of 64 bits, or an int64
     CUDA tensor of one element that is read when the kernel runs (so that a captured graph draws a new mask at each
     replay after the tensor is overwritten); drawn from torch's default CPU generator when not given, so
-    ``torch.manual_seed`` governs it.  In evaluation nothing is dropped.  Differentiable in input and residual."""
+    ``torch.manual_seed`` governs it (refused while a graph is captured: every replay would draw the one mask).  In evaluation
+    nothing is dropped.  Differentiable in input and residual."""
     _on_device("philox_dropout", input)
     if not 0.0 <= p <= 1.0:
         raise ValueError("philox_dropout: p must be in [0, 1], got %r" % (p,))
@@ -99,7 +100,13 @@ def philox_dropout(
         return input if residual is None else torch.ops.mellin.philox_dropout(input, 0.0, 0, None, residual)
     if isinstance(seed, torch.Tensor):
         return torch.ops.mellin.philox_dropout(input, p, 0, seed, residual)
-    seed = int(torch.randint(0, 2 ** 62, (1,)).item()) if seed is None else int(seed) & ((1 << 64) - 1)
+    if seed is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("philox_dropout: a seed drawn while a graph is captured would be every replay's: pass `seed`, "
+                               "a CUDA tensor that is overwritten between replays (or an int, to keep one mask)")
+        seed = int(torch.randint(0, 2 ** 62, (1,)).item())
+    else:
+        seed = int(seed) & ((1 << 64) - 1)
     return torch.ops.mellin.philox_dropout(input, p, seed - (1 << 64) if seed >> 63 else seed, None, residual)
 
 
@@ -198,10 +205,12 @@ class PhiloxDropout(torch.nn.Module):
 class SequenceBlock(torch.nn.Module):
     """``x + dropout(out(recurrence(norm_act(x))))`` on (batch, frames, channels).
 
-    ``forward(x, lens=None, state=None)`` returns ``(output, state)``.  ``streaming``: one way and the norm frame by frame,
+    ``forward(x, lens=None, state=None, seed=None)`` returns ``(output, state)``.  ``streaming``: one way and the norm frame by frame,
     so that feeding a stream in pieces with the state passed on gives what one call over all of it gives; otherwise the
     recurrence runs both ways and the norm's statistics are an utterance's.  Frames behind an utterance's end come out
-    as they went in plus the output layer's bias: finite where ``x`` is, and never read by the next block."""
+    as they went in plus the output layer's bias: finite where ``x`` is, and never read by the next block.  ``seed``: the
+    dropout's, as :func:`philox_dropout` takes it; a captured training step needs it, one for each block (blocks of one shape
+    that share a seed drop the same elements)."""
 
     def __init__(self, channels: int, hidden: Optional[int] = None, num_groups: int = 32, activation: str = "silu",
                  dropout: float = 0.05, streaming: bool = False):
@@ -212,6 +221,7 @@ class SequenceBlock(torch.nn.Module):
         self.out = torch.nn.Linear(hidden * self.recurrence.directions, channels)
         self.dropout = PhiloxDropout(dropout)
 
-    def forward(self, x: torch.Tensor, lens: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None):
+    def forward(self, x: torch.Tensor, lens: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None,
+                seed: Union[None, int, torch.Tensor] = None):
         y, state = self.recurrence(self.norm(x, lens), lens, state)
-        return self.dropout(self.out(y), x), state
+        return self.dropout(self.out(y), x, seed), state

@@ -111,6 +111,51 @@ def test_per_frame_norm_with_lengths():
         norm(x.view(3, 7, 2, 6).reshape(3, 7, 1, 12), lens)
 
 
+def test_block_in_a_captured_step():
+    """A training step of the block captured with a seed on the device: every replay draws the mask of the seed it finds.
+    Without a seed the capture is refused, by the block, the module and the function; in evaluation there is none to draw."""
+    torch.manual_seed(4)
+    block = sequence.SequenceBlock(32, 16, num_groups=4, dropout=0.4).cuda()
+    x, grad = torch.randn(2, 50, 32, device="cuda"), torch.randn(2, 50, 32, device="cuda")
+    seed = torch.tensor(3, device="cuda")
+
+    def step(seed):
+        leaf = x.detach().requires_grad_(True)
+        y, state = block(leaf, seed=seed)
+        return [y.detach(), state.detach()] + list(torch.autograd.grad(y, [leaf] + list(block.parameters()), grad))
+
+    side = torch.cuda.Stream()  # warm-up, as captures of library products want it
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(seed)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(seed)
+    masks = []
+    for k in (3, 4, 2 ** 62 + 1):
+        seed.fill_(k)
+        graph.replay()
+        want = step(k)
+        for got, ref in zip(captured, want):
+            # products may be summed in another order under capture: float32 sums of at most 100 terms of order one
+            assert float((got - ref).abs().max()) <= 1e-4
+        masks.append(captured[0] == x)
+    assert not torch.equal(masks[0], masks[1]) and not torch.equal(masks[1], masks[2])
+    for call in (lambda: block(x), lambda: block.dropout(x), lambda: sequence.philox_dropout(x, 0.4)):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="seed"), torch.no_grad(), torch.cuda.graph(graph):
+            call()
+    block.eval()
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad():
+        want, _ = block(x)
+        with torch.cuda.graph(graph):
+            y, _ = block(x)
+        graph.replay()
+    assert float((y - want).abs().max()) <= 1e-4
+
+
 def test_stream_in_pieces():
     """A streaming block fed 1, 7, 1, 16, ... frames at a time with its state gives what one call gives, to float32
     rounding: sums over 48 channels and states that forget within ~100 frames, some 1e-5 at values of order one."""
