@@ -104,7 +104,7 @@ def philox_dropout(
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("philox_dropout: a seed drawn while a graph is captured would be every replay's: pass `seed`, "
                                "a CUDA tensor that is overwritten between replays (or an int, to keep one mask)")
-        seed = int(torch.randint(0, 2 ** 62, (1,)).item())
+        seed = int(torch.randint(0, 2 ** 62, (1,), device="cpu").item())
     else:
         seed = int(seed) & ((1 << 64) - 1)
     return torch.ops.mellin.philox_dropout(input, p, seed - (1 << 64) if seed >> 63 else seed, None, residual)

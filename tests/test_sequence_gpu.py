@@ -493,6 +493,16 @@ def test_dropout_evaluation_and_defaults():
     assert abs(kept - 0.9) <= 5 * (0.09 / (1 << 20)) ** 0.5
 
 
+def test_dropout_seed_under_a_default_device():
+    """The seed comes from the CPU generator whatever device new tensors go to."""
+    x = torch.randn(4, 50, device="cuda")
+    torch.manual_seed(5)
+    want = sequence.philox_dropout(x, 0.5)
+    torch.manual_seed(5)
+    with torch.device("cuda"):
+        assert torch.equal(sequence.philox_dropout(x, 0.5), want)
+
+
 def test_dropout_offsets_beyond_32_bits():
     """The counter's upper half: elements from 2^34 on (counter 2^32) draw other words than those from 0 on."""
     count = 2 ** 34 + 4096
