@@ -14,6 +14,13 @@ import numpy as np
 STEP = 16.0  # units a step may be off: exp 2 + |argument| <= 8, quotient 2, products and sums 4
 
 
+def gate_step(g):
+    """Units that a step with the sigmoid of ``g`` may be off: the exponential's argument g log2(e) is rounded, and log2(e)
+    itself, which makes 1.22 |g| of them beyond what the eight in STEP cover."""
+    g = np.abs(g)
+    return np.where(g <= 8, STEP, 8 + 1.25 * g)
+
+
 def sigmoid(g):
     with np.errstate(over="ignore"):
         return np.where(g >= 0, 1 / (1 + np.exp(-np.abs(g))), np.exp(-np.abs(g)) / (1 + np.exp(-np.abs(g))))
@@ -23,7 +30,6 @@ def recurrence(x, gate, initial=None, lens=None, reverse=False, grad_y=None, gra
     """Values and bounds: dict of name -> (value, bound).  Frames behind an utterance's end are not looked at."""
     n, t, c = x.shape
     lens = np.full(n, t) if lens is None else np.clip(np.asarray(lens), 0, t)
-    k = STEP * u
     out = {name: (np.zeros((n, t, c)), np.zeros((n, t, c))) for name in ("y", "grad_x", "grad_gate")}
     final = (np.zeros((n, c)), np.zeros((n, c)))
     first = (np.zeros((n, c)), np.zeros((n, c)))
@@ -34,7 +40,7 @@ def recurrence(x, gate, initial=None, lens=None, reverse=False, grad_y=None, gra
         e = np.zeros(c)
         before = {}
         for j in order:
-            f, keep = sigmoid(gate[i, j]), sigmoid(-gate[i, j])
+            f, keep, k = sigmoid(gate[i, j]), sigmoid(-gate[i, j]), gate_step(gate[i, j]) * u
             before[j] = (h, e)
             e = f * e + k * (f * np.abs(h) + keep * np.abs(x[i, j]))
             h = f * h + keep * x[i, j]
@@ -43,7 +49,7 @@ def recurrence(x, gate, initial=None, lens=None, reverse=False, grad_y=None, gra
         m = np.zeros(c) if grad_final is None else grad_final[i].astype(np.float64)
         e = np.zeros(c)
         for j in reversed(order):
-            f, keep = sigmoid(gate[i, j]), sigmoid(-gate[i, j])
+            f, keep, k = sigmoid(gate[i, j]), sigmoid(-gate[i, j]), gate_step(gate[i, j]) * u
             gy = np.zeros(c) if grad_y is None else grad_y[i, j]
             gh, eh = gy + m, e + k * (np.abs(gy) + np.abs(m))
             hb, eb = before[j]

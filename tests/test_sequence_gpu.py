@@ -184,6 +184,35 @@ def test_recurrence_extreme_gates():
         assert torch.isfinite(gx).all() and float(gg.abs().max()) <= 1.01 * least * 480 * 480
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64], ids=str)
+def test_recurrence_sigmoid_and_its_complement(dtype):
+    """Gates up to +-80, one frame: behind a state of 1 and a value of 0 the output is sigmoid(gate), the other way round its
+    complement, each to the step's bound relative to itself (1e-35 at the far end)."""
+    gate = torch.linspace(-80, 80, 200001, device="cuda", dtype=torch.float64).to(dtype).view(1, 1, -1)
+    g, u = _np(gate)[0, 0], _unit(dtype)
+    zero, one = torch.zeros_like(gate), torch.ones_like(gate)
+    f, _ = sequence.gated_recurrence(zero, gate, one[:, 0])
+    keep, _ = sequence.gated_recurrence(one, gate, zero[:, 0])
+    for got, want in ((f, so.sigmoid(g)), (keep, so.sigmoid(-g))):
+        assert (np.abs(_np(got)[0, 0] - want) <= so.gate_step(g) * u * want).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("n,t,c,reverse", [(3, 4, 10, False), (2, 150, 33, True), (2, 150, 64, False), (2, 700, 16, True)])
+def test_recurrence_gates_up_to_80(n, t, c, reverse, dtype):
+    rng = np.random.default_rng(t + c)
+    state = torch.float64 if dtype == torch.float64 else torch.float32
+    x, gate, gy = (torch.from_numpy(v).to("cuda").to(dtype) for v in
+                   (rng.standard_normal((n, t, c)), rng.uniform(-80, 80, (n, t, c)), rng.standard_normal((n, t, c))))
+    initial, gf = (torch.from_numpy(rng.standard_normal((n, c))).to("cuda").to(state) for _ in range(2))
+    want = so.recurrence(_np(x), _np(gate), _np(initial), None, reverse, _np(gy), _np(gf), _unit(dtype))
+    leaves = [v.requires_grad_(True) for v in (x, gate, initial)]
+    y, final = sequence.gated_recurrence(*leaves, reverse=reverse)
+    grads = torch.autograd.grad([y, final], leaves, [gy, gf])
+    for got, name in zip((y, final) + grads, ("y", "final", "grad_x", "grad_gate", "grad_initial")):
+        _close(got, want[name], state if name in ("final", "grad_initial") else dtype, name)
+
+
 @pytest.mark.parametrize("frames", [3, 40, 600])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64], ids=str)
 def test_recurrence_shut_gate_behind_a_huge_state(frames, dtype):
