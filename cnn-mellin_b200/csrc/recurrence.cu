@@ -41,7 +41,7 @@ struct RecurrenceArgs {
 
 // One thread per (utterance, channel), frame after frame: for a few frames a call, where there is nothing to split, and
 // for tensors whose frames lie 2^31 elements or more apart.
-template <typename T, int EVERY>
+template <typename T>
 __global__ void __launch_bounds__(kWalkThreads) recurrence_walk_kernel(const RecurrenceArgs<T> a) {
   begin<false>();
   using A = Acc<T>;
@@ -49,12 +49,12 @@ __global__ void __launch_bounds__(kWalkThreads) recurrence_walk_kernel(const Rec
   if (i >= (long long)a.batch * a.channels) return;
   const long long n = i / a.channels, c = i - n * a.channels;
   const int len = live_frames(a.lens, n, a.frames);
-  const long long slots = (a.frames + EVERY - 1) / EVERY;
+  const long long slots = (a.frames + kStateStride - 1) / kStateStride;
   const T *x = a.x.p + n * a.x.sn + c, *gate = a.gate.p + n * a.gate.sn + c;
   T *y = a.y.p + n * a.y.sn + c;
   A h = a.initial != nullptr ? a.initial[i] : A(0);
   for (int s = 0; s < len; ++s) {
-    if (a.states != nullptr && s % EVERY == 0) a.states[(n * slots + s / EVERY) * a.channels + c] = h;
+    if (a.states != nullptr && s % kStateStride == 0) a.states[(n * slots + s / kStateStride) * a.channels + c] = h;
     const long long t = a.reverse ? len - 1 - s : s;
     A f, keep;
     sigmoid_pair<true>(to_acc(gate[t * a.gate.st]), f, keep);
@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(kWalkThreads) recurrence_walk_kernel(const Rec
   if (a.final != nullptr) a.final[i] = h;
 }
 
-template <typename T, int EVERY>
+template <typename T>
 __global__ void __launch_bounds__(kWalkThreads) recurrence_walk_backward_kernel(const RecurrenceArgs<T> a) {
   begin<false>();
   using A = Acc<T>;
@@ -73,16 +73,16 @@ __global__ void __launch_bounds__(kWalkThreads) recurrence_walk_backward_kernel(
   if (i >= (long long)a.batch * a.channels) return;
   const long long n = i / a.channels, c = i - n * a.channels;
   const int len = live_frames(a.lens, n, a.frames);
-  const long long slots = (a.frames + EVERY - 1) / EVERY;
+  const long long slots = (a.frames + kStateStride - 1) / kStateStride;
   const T *x = a.x.p + n * a.x.sn + c, *gate = a.gate.p + n * a.gate.sn + c;
   const T *gy = a.grad_y.p == nullptr ? nullptr : a.grad_y.p + n * a.grad_y.sn + c;
   T *gx = a.grad_x.p + n * a.grad_x.sn + c, *gg = a.grad_gate.p + n * a.grad_gate.sn + c;
   A m = a.grad_final != nullptr ? a.grad_final[i] : A(0);
-  for (int first = (len - 1) / EVERY * EVERY; len > 0 && first >= 0; first -= EVERY) {
-    A f[EVERY], keep[EVERY], d[EVERY];  // d = h_{t-1} - x_t
-    A h = a.states[(n * slots + first / EVERY) * a.channels + c];
+  for (int first = (len - 1) / kStateStride * kStateStride; len > 0 && first >= 0; first -= kStateStride) {
+    A f[kStateStride], keep[kStateStride], d[kStateStride];  // d = h_{t-1} - x_t
+    A h = a.states[(n * slots + first / kStateStride) * a.channels + c];
 #pragma unroll
-    for (int k = 0; k < EVERY; ++k) {
+    for (int k = 0; k < kStateStride; ++k) {
       if (first + k < len) {
         const long long t = a.reverse ? len - 1 - (first + k) : first + k;
         const A xv = to_acc(x[t * a.x.st]);
@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(kWalkThreads) recurrence_walk_backward_kernel(
       }
     }
 #pragma unroll
-    for (int k = EVERY - 1; k >= 0; --k) {
+    for (int k = kStateStride - 1; k >= 0; --k) {
       if (first + k < len) {
         const long long t = a.reverse ? len - 1 - (first + k) : first + k;
         const A gh = m + (gy != nullptr ? to_acc(gy[t * a.grad_y.st]) : A(0));
@@ -780,14 +780,11 @@ int run(const char *who, RecurrenceArgs<T> a, int64_t batch, int64_t frames, int
     const bool lengthy = is_long(batch, frames, channels);
     auto near = [](const auto &f) { return f.st < 0x7fffffffLL && f.st > -0x7fffffffLL; };
     if (frames <= kWalkFrames || !(near(a.x) && near(a.gate) && near(a.grad_y) && near(a.y) && near(a.grad_x) && near(a.grad_gate))) {
+      if (lengthy)  // 1 TB in 16 bits: no device has them
+        return fail(MELLIN_ERR_UNSUPPORTED, std::string(who) + ": 256 frames or more with 2^31 elements between them");
       const long long blocks = (batch * channels + kWalkThreads - 1) / kWalkThreads;
-      if constexpr (BACKWARD) {
-        if (lengthy) return launch(who, recurrence_walk_backward_kernel<T, kRows>, a, blocks, kWalkThreads, stream);
-        return launch(who, recurrence_walk_backward_kernel<T, kStateStride>, a, blocks, kWalkThreads, stream);
-      } else {
-        if (lengthy) return launch(who, recurrence_walk_kernel<T, kRows>, a, blocks, kWalkThreads, stream);
-        return launch(who, recurrence_walk_kernel<T, kStateStride>, a, blocks, kWalkThreads, stream);
-      }
+      if constexpr (BACKWARD) return launch(who, recurrence_walk_backward_kernel<T>, a, blocks, kWalkThreads, stream);
+      else return launch(who, recurrence_walk_kernel<T>, a, blocks, kWalkThreads, stream);
     }
     if (lengthy) {
       if (packed(a, channels, 2)) return launch_long<T, 2, 8, BACKWARD>(who, a, stream);

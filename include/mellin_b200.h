@@ -312,7 +312,8 @@ int mellin_lift_compress_backward_f64(const double *x, const double *grad_y, con
  * NULL: zeros.  final: receives the state after the last one, or NULL.  states: receives what backward recomputes
  * from, mellin_gated_recurrence_state_count(...) elements, or NULL when no backward call follows.
  * Backward: grad_y and grad_final may be NULL (zeros); grad_initial may be NULL.  grad_x and grad_gate may be the two
- * halves of one tensor; no output may overlap an input. */
+ * halves of one tensor; no output may overlap an input.  Where frames lie 2^31 elements or more apart, fewer
+ * than 256 of them are taken (more have no room on a device). */
 int64_t mellin_gated_recurrence_state_count(int64_t batch, int64_t frames, int64_t channels);
 int mellin_gated_recurrence_f32(const float *x, int64_t x_sn, int64_t x_st, const float *gate, int64_t gate_sn,
                                 int64_t gate_st, const float *initial, const int *lens, int reverse, int64_t batch,

@@ -246,6 +246,25 @@ def test_recurrence_strides_beyond_32_bits():
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("reverse", [False, True])
+def test_recurrence_frames_2_to_31_apart(reverse):
+    """Frames beyond what a 32-bit step reaches: the form of one thread per channel, both ways."""
+    far, dtype = 2 ** 31, torch.bfloat16
+    flat = torch.empty(4 * far + 96, dtype=dtype, device="cuda")
+    rng = np.random.default_rng(17)
+    small = [torch.from_numpy(rng.standard_normal((1, 5, 32))).to("cuda").to(dtype) for _ in range(3)]
+    x, gate, gy = (flat[32 * k:].as_strided((1, 5, 32), (0, far, 1)) for k in range(3))
+    for v, w in zip((x, gate, gy), small):
+        v.copy_(w)
+    initial, gf = (torch.from_numpy(rng.standard_normal((1, 32))).to("cuda").float() for _ in range(2))
+    want = so.recurrence(*(_np(v) for v in (small[0], small[1], initial)), None, reverse, _np(small[2]), _np(gf))
+    leaves = [v.detach().requires_grad_(True) for v in (x, gate, initial)]
+    y, final = sequence.gated_recurrence(*leaves, reverse=reverse)
+    grads = torch.autograd.grad([y, final], leaves, [gy, gf])
+    for got, name in zip((y, final) + grads, ("y", "final", "grad_x", "grad_gate", "grad_initial")):
+        _close(got, want[name], torch.float32 if name in ("final", "grad_initial") else dtype, name)
+
+
 def test_recurrence_empty():
     for shape in ((0, 5, 8), (2, 0, 8), (2, 5, 0)):
         x = torch.randn(*shape, device="cuda", requires_grad=True)

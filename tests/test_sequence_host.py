@@ -164,3 +164,18 @@ def test_statistics_offsets_beyond_32_bits(tmp_path):
     text = open(os.path.join(csrc, "group_norm.cu")).read()
     uses = re.findall(r"a\.stats(?:_out)? \+ (\w+)|a\.stats(?:_out)?(\[)", text)
     assert len(uses) == 5 and all(use == ("stats_offset", "") for use in uses)
+
+
+@pytest.mark.parametrize("sfx", ["_f32", "_f64", "_f16", "_bf16"])
+def test_recurrence_refuses_what_no_device_holds(sfx):
+    """256 frames that lie 2^31 elements apart: refused before anything is launched (the pointers are no memory)."""
+    lib, at, far = capi.lib(), ctypes.c_void_p(4096), 2 ** 31
+    dense = [at, I64(300 * 8), I64(8)]
+    for forward in ([at, I64(0), I64(far)] + dense + [NULL, NULL, 0, I64(1), I64(300), I64(8)] + dense,
+                    dense + [at, I64(0), I64(far)] + [NULL, NULL, 1, I64(1), I64(300), I64(8)] + dense,
+                    dense + dense + [NULL, NULL, 0, I64(1), I64(300), I64(8)] + [at, I64(0), I64(far)]):
+        assert getattr(lib, "mellin_gated_recurrence" + sfx)(*forward, NULL, NULL, NULL) == UNSUPPORTED
+        assert b"between them" in lib.mellin_last_error()
+    back = getattr(lib, "mellin_gated_recurrence_backward" + sfx)
+    assert back(*dense, *dense, at, NULL, 0, I64(1), I64(300), I64(8), at, I64(0), I64(far), NULL, *dense, *dense, NULL,
+                NULL) == UNSUPPORTED
