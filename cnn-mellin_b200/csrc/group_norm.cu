@@ -10,6 +10,11 @@
 //   gx = rstd * (weight gz - (sum_c weight P1 + xhat * sum_c weight P2) / M)
 //
 // All sums in a fixed order: two runs give the same bits.
+//
+// ReLU's slope is 1 where z as computed is positive.  z next to zero is the difference of terms as large as the bias, so in
+// float which side it falls on is certain to about 2e-8: of 16.4 million elements (32 utterances of 200 to 800 frames, 1024
+// channels) one was on the other side than in 64 bits in 11 of 120 draws, never at |z| above 2.2e-8; the same formula written
+// out in elementary operations, 15 of 120.  Statistics rounded to float alone would leave 7.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -350,6 +350,47 @@ def test_group_norm_act(case, dtype):
         assert torch.equal(sequence.group_norm_act(x, groups, weight, bias, lens_d, 1e-5, act), y)
 
 
+def test_relu_slope_at_the_training_size():
+    """32 utterances of 200 to 800 frames and 1024 channels: every gradient against float64, and every side of ReLU's corner
+    that is not the one of 64 bits lies within float32's rounding of it.
+
+    z = (x - mean) * (rstd * weight) + bias: near the corner the two terms are as large as the bias.  mean is off by a few
+    units of the values (2^-24 * 0.5), rstd by a few of its own, the factor and the product by half a unit each: below 16
+    units of |bias| + |mean * rstd * weight|, some 2e-6.  With grad_y zero wherever |z| is below that no gradient depends on
+    the side, and what is left is rounding: single terms to 16 units, sums of up to 25600 terms by trees."""
+    n, t, c, groups = 32, 800, 1024, 32
+    lens = torch.tensor([200 + 600 * (7 * i % 32) // 31 for i in range(n)], dtype=torch.int32, device="cuda")
+    for seed in range(4):
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        x = torch.randn(n, t, c, device="cuda", generator=gen).mul_(1.5).add_(0.5)
+        w = torch.randn(c, device="cuda", generator=gen).mul_(0.2).add_(1)
+        b = torch.randn(c, device="cuda", generator=gen).mul_(0.2)
+        gy = torch.randn(n, t, c, device="cuda", generator=gen)
+        wd, bd = w.double(), b.double()
+        y = sequence.group_norm_act(x, groups, w, b, lens)
+        want = [torch.zeros(n, t, c, device="cuda", dtype=torch.float64)] + [torch.zeros_like(wd) for _ in range(2)]
+        for i in range(n):
+            length = int(lens[i])
+            v = x[i, :length].double().view(length, groups, -1)
+            mean = v.mean((0, 2), keepdim=True)
+            rstd = ((v - mean).square().mean((0, 2), keepdim=True) + 1e-5).rsqrt()
+            xhat = ((v - mean) * rstd).view(length, c)
+            z = xhat * wd + bd
+            around = (mean.abs() * rstd).expand(1, groups, c // groups).reshape(c) * wd.abs() + bd.abs()
+            near = z.abs() <= 16 * 2 ** -24 * around
+            assert not bool((((y[i, :length] > 0) != (z > 0)) & ~near).any())
+            gy[i, :length].masked_fill_(near, 0)
+            gz = gy[i, :length].double() * (z > 0)
+            want[1] += (gz * xhat).sum(0)
+            want[2] += gz.sum(0)
+            q, h = (gz * wd).view(length, groups, -1), xhat.view(length, groups, -1)
+            want[0][i, :length] = (rstd * (q - q.mean((0, 2), keepdim=True) - h * (q * h).mean((0, 2), keepdim=True))).view(length, c)
+        leaves = [v.requires_grad_(True) for v in (x, w, b)]
+        got = torch.autograd.grad(sequence.group_norm_act(x, groups, w, b, lens), leaves, gy)
+        for g, ref in zip(got, want):
+            assert float((g - ref).norm() / ref.norm()) <= 1e-6
+
+
 def test_group_norm_large_mean():
     """Values far from zero: the variance is taken from deviations, not as a difference of squares.
 
@@ -477,6 +518,30 @@ def test_many_utterances():
     h, _ = sequence.gated_recurrence(x.detach().expand(140001, 9, 16), gy.expand(140001, 9, 16))
     h2, _ = sequence.gated_recurrence(x.detach()[139000:].expand(1001, 9, 16), gy[139000:].expand(1001, 9, 16))
     assert torch.equal(h[139000:], h2)
+
+
+def test_parameter_sums_of_many_utterances():
+    """Parameter gradients over more utterances than a grid's second extent has blocks, against float64.
+
+    Rounding: a channel's sum wanders within some sqrt(140001) = 374 (terms of order one, either sign), rounded at most 300
+    times on the way of one value (the utterances a block takes, the sets, the join): 2^-24 * 374 * sqrt(300) = 4e-4; the
+    terms themselves are off by some 8 units each: 8 * 2^-24 * 374 = 2e-4.  1e-2 leaves a factor of 16; a single utterance that
+    is lost or taken twice moves the 16 channels by terms of order one (checked for a few of them)."""
+    gen = torch.Generator(device="cuda").manual_seed(16)
+    n, c = 140001, 16
+    x, gy = (torch.randn(n, 1, c, device="cuda", generator=gen) for _ in range(2))
+    w, b = (torch.randn(c, device="cuda", generator=gen) for _ in range(2))
+    leaves = [v.requires_grad_(True) for v in (x, w, b)]
+    got = torch.autograd.grad(sequence.group_norm_act(x, 2, w, b, activation="silu"), leaves, gy)
+    v = x.detach().double().view(n, 2, c // 2)
+    d = v - v.mean(2, keepdim=True)
+    xhat = (d / (d.square().mean(2, keepdim=True) + 1e-5).sqrt()).view(n, c)
+    z = xhat * w.detach().double() + b.detach().double()
+    s = torch.sigmoid(z)
+    gz = gy.view(n, c).double() * s * (1 + z * (1 - s))
+    for g, terms in ((got[1], gz * xhat), (got[2], gz)):
+        assert float((g - terms.sum(0)).abs().max()) <= 1e-2
+        assert all(float(terms[i].abs().max()) > 2e-2 for i in (0, 65534, 65535, 131070, n - 1))
 
 
 def test_group_norm_strides_beyond_32_bits():
