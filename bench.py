@@ -30,8 +30,9 @@ front of the first layer as one pass, against the HBM roofline and against the
 stock torch operators; single-GPU runs only).
 
 With ``--impl reference`` the headline step is run by the reference's own CPU
-kernels (``oracle/_ref``, OpenMP over all host cores; the C restatement when
-that library is absent) on the full batch, for the steps asked for.
+kernels (``oracle/_ref``, OpenMP over all host cores) on the full batch, for
+the steps asked for; where that library could not be built the arm says so and
+measures nothing (the C restatement is not the reference).
 
 Multi-GPU (torchrun, one rank per GPU): every rank runs its own batch-32 shard
 (weak scaling); the weight and bias gradients land directly in a flat bucket
@@ -220,6 +221,12 @@ def run_reference(args):
     """The reference's CPU implementation of the same step, same batch, on the host cores."""
     rank = int(os.environ.get("RANK", "0"))
     if rank != 0:
+        return
+    from oracle.oracle import Oracle
+
+    if not Oracle.reference_available():
+        print(json.dumps({"impl": "reference", "unavailable": "the reference has no package to install, and oracle/_ref, its "
+                          "CPU kernels compiled from a checkout, is not there"}), flush=True)
         return
     step, kind, cores = _cpu_step_factory()
     budget_s = 150.0  # the whole arm must end within a few minutes whatever K is
