@@ -1,7 +1,7 @@
 // Dropout whose mask is a function of (seed, element offset) and is never stored, with an optional residual added in the
 // same pass:
 //
-//   y[i] = (word(i) >= p * 2^32 ? x[i] / (1 - p) : 0) + residual[i]
+//   y[i] = (word(i) >= round(p * 2^32) ? x[i] / (1 - p) : 0) + residual[i]
 //
 // word(i) is word i % 4 of Philox4x32-10 (J. K. Salmon, M. A. Moraes, R. O. Dror, D. E. Shaw: Parallel random numbers:
 // as easy as 1, 2, 3; SC 2011) with counter i / 4 and the 64-bit seed as key, i the element's offset in row-major order.
@@ -39,8 +39,8 @@ struct DropoutArgs {
   const T *x = nullptr, *residual = nullptr;  // residual may be null
   T *y = nullptr;
   long long rows = 0, cols = 0, x_stride = 0, r_stride = 0;  // y is dense; strides between rows, in elements
-  bool drop = false;       // p > 0; without it no word is drawn
-  unsigned threshold = 0;  // kept where word > threshold = p * 2^32 - 1
+  bool drop = false;       // round(p * 2^32) > 0; without it no word is drawn
+  unsigned threshold = 0;  // kept where word > threshold = round(p * 2^32) - 1
   Acc<T> scale = 1;
   unsigned long long seed = 0;
   const long long *seed_device = nullptr;  // read instead of `seed` when there is one
@@ -105,6 +105,9 @@ __global__ void __launch_bounds__(kThreads) philox_dropout_kernel(const DropoutA
         const Words w = philox4x32_10((unsigned long long)(i / 4 + g), key);
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[g * 4 + j] = w.w[j] > a.threshold ? x[g * 4 + j] * a.scale : A(0);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[g * 4 + j] *= a.scale;  // 1, or what double sees of a p that drops nothing
       }
       if constexpr (RESIDUAL) {
 #pragma unroll

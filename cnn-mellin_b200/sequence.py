@@ -89,7 +89,7 @@ def philox_dropout(
     """Dropout, plus ``residual`` when given; the mask is a function of ``seed`` and of an element's offset.
 
     Element ``i`` (row-major offset) is dropped where word ``i % 4`` of Philox4x32-10 at counter ``i // 4`` with key
-    ``seed`` is below ``p * 2**32``; the others are scaled by ``1 / (1 - p)``.  The mask is never stored: backward draws
+    ``seed`` is below ``floor(p * 2**32 + 0.5)``; the others are scaled by ``1 / (1 - p)``.  The mask is never stored: backward draws
     it again.  A dropped element is zero whatever ``input`` holds there.  ``seed``: an integer of 64 bits, or an int64
     CUDA tensor of one element that is read when the kernel runs (so that a captured graph draws a new mask at each
     replay after the tensor is overwritten); drawn from torch's default CPU generator when not given, so

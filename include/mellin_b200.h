@@ -413,7 +413,7 @@ int mellin_group_norm_act_backward_bf16(const void *x, int64_t x_sn, int64_t x_s
                                        size_t workspace_bytes, void *stream);
 
 /* Dropout with a mask that is a function of (seed, element offset): element i (row-major offset) is dropped where word
- * i % 4 of Philox4x32-10 with counter i / 4 and key `seed` is below p * 2^32, and scaled by 1 / (1 - p) otherwise;
+ * i % 4 of Philox4x32-10 with counter i / 4 and key `seed` is below round(p * 2^32), and scaled by 1 / (1 - p) otherwise;
  * residual (or NULL) is added.  A dropped element is zero whatever x holds.  x and residual are (rows, cols) with
  * *_stride elements between rows; y is dense.  seed_device (or NULL) is a device word read instead of `seed`, so that
  * a captured graph can draw a new mask at each replay.  Backward: the same call on the gradient, without residual. */

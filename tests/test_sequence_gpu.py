@@ -606,6 +606,21 @@ def test_dropout_evaluation_and_defaults():
     assert abs(kept - 0.9) <= 5 * (0.09 / (1 << 20)) ** 0.5
 
 
+def test_dropout_probabilities_at_the_words_resolution():
+    """Probabilities next to a whole number of 2^-32, and below one of them: the words are compared with the nearest whole
+    number, the kept elements scaled by what is asked for."""
+    x = torch.randn(1 << 16, device="cuda", dtype=torch.float64, requires_grad=True)
+    words = so.philox4x32_10(np.arange(1 << 14), 5).reshape(-1)
+    at = float(int(words[1000]))  # a word that lies on the border
+    for p in (1e-11, 2.0 ** -34, at * 2.0 ** -32, (at + 0.49) * 2.0 ** -32, (at + 0.51) * 2.0 ** -32, 1 - 2.0 ** -40):
+        keep = so.dropout_keep((1 << 16,), p, 5)
+        y = sequence.philox_dropout(x, p, True, 5)
+        g, = torch.autograd.grad(y.sum(), x)
+        for got, ref in ((y, np.where(keep, _np(x) / (1 - p), 0)), (g, keep / (1 - p))):
+            assert (np.abs(_np(got) - ref) <= 2 * 2.0 ** -53 * np.abs(ref)).all(), p
+    assert so.dropout_keep((1 << 16,), at * 2.0 ** -32, 5)[1000] and not so.dropout_keep((1 << 16,), (at + 0.51) * 2.0 ** -32, 5)[1000]
+
+
 def test_dropout_seed_under_a_default_device():
     """The seed comes from the CPU generator whatever device new tensors go to."""
     x = torch.randn(4, 50, device="cuda")
