@@ -254,6 +254,7 @@ std::tuple<Tensor, Tensor> norm_forward(const Tensor &input, int64_t groups, con
   const int64_t n = input.size(0), t = input.size(1), channels = input.size(2);
   TORCH_CHECK(groups > 0 && channels % groups == 0, c, ": ", channels, " channels do not divide into ", groups, " groups");
   TORCH_CHECK(eps >= 0, c, ": 'eps' must not be negative");
+  TORCH_CHECK(act >= 0 && act <= 3, c, ": unknown activation ", act);
   if (weight) check_like(c, *weight, "weight", input, {channels});
   if (bias) check_like(c, *bias, "bias", input, {channels});
   check_lens(c, lens_in, input);

@@ -736,6 +736,14 @@ def test_refusals():
         y.sum().backward()
 
 
+def test_unknown_activation_numbers():
+    """The operator's own argument is a 64-bit number: one whose lower half names an activation is none."""
+    x = torch.randn(2, 4, 6, device="cuda")
+    for act in (4, -1, 2 ** 32, 2 ** 32 + 1):
+        with pytest.raises(RuntimeError, match="unknown activation"):
+            torch.ops.mellin.group_norm_act(x, 2, act=act)
+
+
 @pytest.mark.parametrize("frames", [3, 40, 2600])
 def test_other_stream_and_captured_graph(frames):
     """The same results on a stream of the caller's, and from a graph that is replayed on other inputs: at a few frames, at
