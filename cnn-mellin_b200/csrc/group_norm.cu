@@ -897,6 +897,7 @@ int run_forward(NormArgs<T> a, int64_t batch, int64_t frames, int64_t channels, 
                 void *workspace, size_t workspace_bytes, void *stream) {
   const char *who = "group_norm_act";
   return guarded(who, [&]() -> int {
+    if (!(eps >= 0)) return fail(MELLIN_ERR_BAD_ARGUMENT, std::string(who) + ": eps must not be negative or NaN");
     int rc = prepare(who, a, batch, frames, channels, groups, act, false, workspace, workspace_bytes);
     if (rc != MELLIN_OK || batch == 0 || channels == 0) return rc;
     if (frames > 0 && (a.x.p == nullptr || a.y.p == nullptr))

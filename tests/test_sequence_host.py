@@ -179,3 +179,13 @@ def test_recurrence_refuses_what_no_device_holds(sfx):
     back = getattr(lib, "mellin_gated_recurrence_backward" + sfx)
     assert back(*dense, *dense, at, NULL, 0, I64(1), I64(300), I64(8), at, I64(0), I64(far), NULL, *dense, *dense, NULL,
                 NULL) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("sfx", ["_f32", "_f64", "_f16", "_bf16"])
+def test_norm_refuses_a_bad_epsilon(sfx):
+    lib = capi.lib()
+    for eps in (-1e-5, float("nan"), float("-inf")):
+        assert getattr(lib, "mellin_group_norm_act" + sfx)(
+            NULL, I64(0), I64(0), NULL, NULL, NULL, I64(0), I64(4), I64(6), I64(3), ctypes.c_double(eps), 0, NULL, I64(0),
+            I64(0), NULL, NULL, ctypes.c_size_t(0), NULL) == BAD
+        assert b"eps" in lib.mellin_last_error()
