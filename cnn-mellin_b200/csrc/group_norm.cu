@@ -134,7 +134,7 @@ constexpr A kGrow = A(4294967296.0);
 // memory, all copies issued at once, so x (and grad_y) is read once.  Teams are as small as the group allows, down to
 // four threads, so that groups of a single frame share a warp.  Bound by HBM: two or more blocks a multiprocessor overlap one's sums
 // with another's loads and stores.  Measured with 32 utterances of 200 to 800 frames, 1024 channels, 32 groups: float32
-// and ReLU 37 us forward and 55 us backward (bytes alone: 26 and 36), bfloat16 and SiLU 27 and 47 (13 and 18: the special
+// and ReLU 32 us forward and 55 us backward (bytes alone: 26 and 36), bfloat16 and SiLU 26 and 43 (13 and 18: the special
 // function unit and the conversions count there).  Values kept in registers instead, 64 a thread: 68 and 151 us (fewer
 // bytes in flight, more clusters, code beyond the instruction cache).  Utterances are taken as they come: sorting them
 // costs every block more than the shorter tail gains (float32 backward 60 us).
@@ -480,7 +480,7 @@ __device__ __forceinline__ void add_parts(const NormArgs<T> &a, int parts, int b
 // of its utterance's frames; `slabs` blocks side by side have a frame of the group, `chunks` one after the other its
 // frames.  The first launch writes every block's sums; in the second every
 // block adds its group's and normalises its part, read from L2 as a rule.  4 x 16384 x 256 channels, 8 groups, SiLU,
-// bfloat16: 25 us forward and 42 us backward (bytes alone: 10 and 15); 12 x 548..2191 x 549 float32, one group: 39 and 55
+// bfloat16: 26 us forward and 44 us backward (bytes alone: 10 and 15); 12 x 548..2191 x 549 float32, one group: 39 and 55
 // (12 and 22).
 
 // frames of a thread fetched together: 8, or 4 where two tensors of 16 bytes a thread would fill the registers (four with

@@ -46,10 +46,11 @@ struct DropoutArgs {
   const long long *seed_device = nullptr;  // read instead of `seed` when there is one
 };
 
-// Two accesses of 16 bytes a thread are in flight before the generator's work, which then bounds 16-bit tensors: a call for
-// four elements has 38 instructions of the multiplier's pipe and 47 of the integer pipe, each of which takes one every
-// second clock.  26.2 M elements: float32 37 us = 5670 GB/s (0.87 of the measured copy rate), bfloat16 32 us = 3230 GB/s,
-// with a residual 37 us = 4240 GB/s.  With whole 64-bit products 40 / 33 / 41 us; with one or four groups a thread 43 / 35 /
+// Two accesses of 16 bytes a thread are in flight before the generator's work, which is half of 16-bit tensors' time: a call
+// for four elements has 38 instructions of the multiplier's pipe and 47 of the integer pipe, each of which takes one every
+// second clock, 17 us of 26.2 M elements.  The other half is the beginning and end of blocks, which others cover in part only
+// (integer pipe busy 60 %, issue slots 65 %).  26.2 M elements: float32 36 us = 5830 GB/s (0.89 of the measured copy rate),
+// bfloat16 31 us = 3380 GB/s, with a residual 37 us = 4240 GB/s.  With whole 64-bit products 40 / 33 / 41 us; with one or four groups a thread 43 / 35 /
 // 40 and 41 / 34 / 41 us.
 //
 // V elements a group, a multiple of 4; U groups a thread, kThreads groups apart, whose loads are issued together.  VEC:

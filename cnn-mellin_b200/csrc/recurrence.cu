@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(32 * W, MB) recurrence_scan_backward_kernel(co
 // is formed by walking it once; these are joined in the warp, the block and the cluster, one exchange in all; then the
 // run is walked again from the state that is now known.  The second walk finds its inputs in L2 (so few utterances and
 // channels are small), and no step waits for another block, as the single walk above would have to every SPAN frames.
-// 16384 frames of 2 x 256 channels in bfloat16: 24 us forward, 33 us backward (bytes alone: 8 and 13); 31 and 41 with
+// 16384 frames of 2 x 256 channels in bfloat16: 26 us forward, 31 us backward (bytes alone: 8 and 13); 31 and 41 with
 // the single walk and an exchange in the cluster every 1024 frames; 37 and 47 with 32 channels a cluster, which leaves
 // half the multiprocessors without one.
 
@@ -791,13 +791,13 @@ int run(const char *who, RecurrenceArgs<T> a, int64_t batch, int64_t frames, int
       return launch_long<T, 1, 16, BACKWARD>(who, a, stream);
     }
     // V, CL, W and blocks a multiprocessor, measured at 32 utterances of 200 to 800 frames and 1024 channels (us, forward
-    // / backward): 16 bits <4, 16, 4, 4> 30 / 73, <4, 16, 4, 2> 35 / 47, <4, 8, 4, 4> 31 / 47, <4, 16, 8, 2> 29 / 66 (39
+    // / backward): 16 bits <4, 16, 4, 4> 30 / 73, <4, 16, 4, 2> 35 / 47, <4, 8, 4, 4> 31 / 45, <4, 16, 8, 2> 29 / 66 (39
     // against 35 forward where all have 800 frames); float <4, 8, 4, 4> 44 / 78, <4, 8, 4, 3> 50 / 77, <4, 16, 4, 2>
-    // 45 / 71.  Bytes alone: 18 / 31 and 36 / 62.  What is left goes to the joins (a barrier every step), to 26
+    // 45 / 68.  Bytes alone: 18 / 31 and 36 / 62.  What is left goes to the joins (a barrier every step), to 26
     // instructions an element, and to 3.5 blocks a multiprocessor; packed multiply-adds changed nothing.
     constexpr int V = sizeof(T) == 8 ? 2 : 4;
     if (!packed(a, channels, V)) {
-      // an even number of channels: pairs, bfloat16 33 / 49; else one by one, 41 / 86
+      // an even number of channels: pairs, 16 bits 35 / 53; else one by one, 44 / 86
       if (V > 2 && packed(a, channels, 2)) return launch_scan<T, 2, 16, 4, 4, BACKWARD>(who, a, stream);
       return launch_scan<T, 1, 32, 4, BACKWARD ? 3 : 4, BACKWARD>(who, a, stream);
     }

@@ -70,9 +70,9 @@ def group_norm_act(
     ``"none"``, ``"relu"``, ``"silu"`` or ``"gelu"`` (with the error function).  Differentiable in input, weight and bias;
     the parameters' gradients are summed in a fixed order.  ReLU's slope is that of the side on which its argument falls as
     computed in float32; where 64 bits have the argument within about 2e-8 of zero that may be the other side (one of 16
-    million elements, in one call of ten), and a parameter's gradient then differs by that element's whole term.  A group whose squared deviations pass the statistics' type
-    (float32 ends at 3.4e38) has no finite variance and comes out as NaN or ``act(bias)``.  Batch times channels is below
-    2^31."""
+    million elements, in one call of ten), and a parameter's gradient then differs by that element's whole term.
+    A group whose squared deviations pass the statistics' type (float32 ends at 3.4e38) has no finite variance and comes out
+    as NaN or ``act(bias)``.  Batch times channels is below 2^31."""
     _on_device("group_norm_act", input)
     if activation not in ACTIVATIONS:
         raise ValueError("group_norm_act: activation must be one of %s, got %r" % (sorted(ACTIVATIONS), activation))

@@ -357,8 +357,8 @@ int mellin_gated_recurrence_backward_bf16(const void *x, int64_t x_sn, int64_t x
                                          int64_t grad_gate_st, float *grad_initial, void *stream);
 
 /* Group norm and an activation: y = act((x - mean) * rstd * weight[c] + bias[c]); mean and biased variance over an
- * utterance's frames and the channels / groups adjacent channels of a group, rstd = 1 / sqrt(var + eps), eps >= 0.  weight / bias:
- * (channels), or NULL: ones / zeros.  act: 0 none, 1 ReLU, 2 SiLU (z sigmoid(z)), 3 GELU (z Phi(z)).  stats: receives
+ * utterance's frames and the channels / groups adjacent channels of a group, rstd = 1 / sqrt(var + eps), eps >= 0.
+ * weight / bias: (channels), or NULL: ones / zeros.  act: 0 none, 1 ReLU, 2 SiLU (z sigmoid(z)), 3 GELU (z Phi(z)).  stats: receives
  * (batch, groups, 2) mean and rstd for backward, or NULL.  workspace: mellin_group_norm_act_workspace_bytes_*() bytes
  * (backward: 0 for a forward call, 1 for a backward call), 16-byte aligned; NULL where that is 0.  Its contents are
  * clobbered.  Backward: grad_weight / grad_bias (channels) may be
