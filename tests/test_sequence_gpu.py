@@ -544,6 +544,26 @@ def test_parameter_sums_of_many_utterances():
         assert all(float(terms[i].abs().max()) > 2e-2 for i in (0, 65534, 65535, 131070, n - 1))
 
 
+def test_group_norm_statistics_beyond_2_to_31():
+    """2^30 + 1024 groups of all utterances, so that the statistics have more than 2^31 elements: the last utterances get what
+    they get in a call of their own, forward and backward."""
+    n, c = 2 ** 20 + 1, 1024
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    last = torch.randn(5, 2, c, device="cuda", generator=gen).bfloat16()
+    x, gy = (torch.zeros(n, 2, c, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    where = [0, 524287, 524288, n - 2, n - 1]
+    for i, k in enumerate(where):
+        x[k], gy[k] = last[i], last[4 - i]
+    x.requires_grad_(True)
+    y = sequence.group_norm_act(x, c, activation="silu")
+    gx, = torch.autograd.grad(y, x, gy)
+    small = last.clone().requires_grad_(True)
+    want = sequence.group_norm_act(small, c, activation="silu")
+    want_x, = torch.autograd.grad(want, small, last.flip(0))
+    assert torch.equal(y[where], want) and torch.equal(gx[where], want_x)
+    assert int(torch.count_nonzero(y)) == int(torch.count_nonzero(want))
+
+
 def test_group_norm_strides_beyond_32_bits():
     flat = torch.zeros(5 * 2 ** 30 + 64, dtype=torch.bfloat16, device="cuda")
     x = flat.as_strided((1, 6, 32), (0, 2 ** 30, 1))
