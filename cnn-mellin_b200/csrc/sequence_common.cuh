@@ -253,9 +253,9 @@ __device__ __forceinline__ double max_nan(double a, double b) { return a > b ? a
 
 // sigmoid(g) and 1 - sigmoid(g), each to 8 + 1.25 |g| units of 2^-24 relative to itself at most: the complement is
 // e sigmoid(g) with e = exp(-g), not a difference, and e is as exact as the product of g and log2(e) is after its rounding to
-// one float (63 units at |g| = 80 as emulated).  e is held at 2^126, so that the quotient stays a normal number (the least sigmoid is
-// 2^-126); NaN stays NaN.  SHUT: where e is held, sigmoid is 0, so that a shut gate lets nothing of a state through whatever
-// its size (2^-126 of 3e38 would be 4); 1 % of the recurrence's time.
+// one float (63 units at |g| = 80 as emulated).  e is held at 2^126, so that the quotient stays a normal number (the least
+// sigmoid is 2^-126); NaN stays NaN.  SHUT: where e is held, sigmoid is 0, so that a shut gate lets nothing of a state
+// through whatever its size (2^-126 of 3e38 would be 4); 1 % of the recurrence's time.
 template <bool SHUT = false>
 __device__ __forceinline__ void sigmoid_pair(float g, float &f, float &keep) {
   float t;

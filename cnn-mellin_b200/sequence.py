@@ -89,8 +89,8 @@ def philox_dropout(
     """Dropout, plus ``residual`` when given; the mask is a function of ``seed`` and of an element's offset.
 
     Element ``i`` (row-major offset) is dropped where word ``i % 4`` of Philox4x32-10 at counter ``i // 4`` with key
-    ``seed`` is below ``floor(p * 2**32 + 0.5)``; the others are scaled by ``1 / (1 - p)``.  The mask is never stored: backward draws
-    it again.  A dropped element is zero whatever ``input`` holds there.  ``seed``: an integer of 64 bits, or an int64
+    ``seed`` is below ``floor(p * 2**32 + 0.5)``; the others are scaled by ``1 / (1 - p)``.  The mask is never stored:
+    backward draws it again.  A dropped element is zero whatever ``input`` holds there.  ``seed``: an integer of 64 bits, or an int64
     CUDA tensor of one element that is read when the kernel runs (so that a captured graph draws a new mask at each
     replay after the tensor is overwritten); drawn from torch's default CPU generator when not given, so
     ``torch.manual_seed`` governs it (refused while a graph is captured: every replay would draw the one mask).  In evaluation
@@ -207,8 +207,8 @@ class PhiloxDropout(torch.nn.Module):
 class SequenceBlock(torch.nn.Module):
     """``x + dropout(out(recurrence(norm_act(x))))`` on (batch, frames, channels).
 
-    ``forward(x, lens=None, state=None, seed=None)`` returns ``(output, state)``.  ``streaming``: one way and the norm frame by frame,
-    so that feeding a stream in pieces with the state passed on gives what one call over all of it gives; otherwise the
+    ``forward(x, lens=None, state=None, seed=None)`` returns ``(output, state)``.  ``streaming``: one way and the norm frame
+    by frame, so that feeding a stream in pieces with the state passed on gives what one call over all of it gives; otherwise the
     recurrence runs both ways and the norm's statistics are an utterance's.  Frames behind an utterance's end come out
     as they went in plus the output layer's bias: finite where ``x`` is, and never read by the next block.  ``seed``: the
     dropout's, as :func:`philox_dropout` takes it; a captured training step needs it, one for each block (blocks of one shape
